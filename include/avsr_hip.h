@@ -542,6 +542,64 @@ int avsr_adamw_step_dev(avsr_stream_t stream, float* param, float* grad, float* 
                         void* bf16_shadow, int64_t n, const float* hyper, float beta1, float beta2, float eps,
                         float weight_decay, const float* grad_scale, int clear_grad, float* clip_scale_reset);
 
+/* ------------------------------------------------------------------------
+ * Serving the Whisper decoder (hf modeling_whisper.py:649-797 with past_key_values) to requests of different lengths
+ * that come and go.  The keys and values of `page` tokens of one layer form a page: element (p, h, t, d) at
+ * pages + p*page_stride + h*head_stride + t*head_dim + d.  page: 16, 32, 64, 128 or 256; head_dim: 64 or 128.
+ * A request holds its pages in a row of a block table (int32, ld_table >= width), token j in entry j / page.
+ *
+ * avsr_paged_plan: the tables of one step, from the requests' lengths, on the GPU.  add[b] >= 0: request b adds that
+ * many tokens to the lens[b] it holds; add[b] < 0: it ends and gives its pages back.  Free pages are a ring of n_pages
+ * entries, pool = {head, count}: pages are taken at the head in the order of requests and positions, and given back
+ * behind the last free one.  Writes the new entries of `table`, the returned ones of `ring`, lens_out [B] (0 for a
+ * request that ended), pool_out [2], q_start [B+1] (first row of each request's new tokens, and their number), and for
+ * the max_tokens rows of the step slots (page * `page` + place in it; -1 behind the last token) and positions (0 there).
+ * All or nothing: status = 0, or a sum of 1 (too few free pages), 2 (a request outgrows its table row), 4 (more tokens
+ * than max_tokens), 8 (a negative length, or a pool that cannot be), and then tables, ring, lengths and pool stay as
+ * they are, q_start is all 0 and slots all -1, so that what follows in the step does nothing.  lens_out may be lens and
+ * pool_out may be pool.  Workspace: avsr_paged_plan_workspace_bytes (0: none). */
+int64_t avsr_paged_plan_workspace_bytes(int64_t B, int64_t max_tokens);
+int avsr_paged_plan(avsr_stream_t stream, const int32_t* lens, const int32_t* add, int32_t* table, int64_t ld_table,
+                    int64_t width, int32_t* ring, int64_t n_pages, const int32_t* pool, int64_t B, int64_t page,
+                    int64_t max_tokens, int32_t* lens_out, int32_t* pool_out, int32_t* q_start, int32_t* slots,
+                    int32_t* positions, int32_t* status, void* workspace);
+/* New keys and values k, v [rows, H, head_dim] (row stride ld, head stride *_head) into the slots of the pages, rounded
+ * once if the pages are bf16 and k, v fp32.  A row whose slot is negative or beyond the pages is left out; slots are
+ * distinct (of two equal ones either row's values may end up in any part of the slot). */
+int avsr_paged_write(avsr_stream_t stream, int in_dtype, int page_dtype, const void* k, int64_t ldk, int64_t k_head,
+                     const void* v, int64_t ldv, int64_t v_head, void* k_pages, int64_t k_page_stride,
+                     int64_t k_head_stride, void* v_pages, int64_t v_page_stride, int64_t v_head_stride,
+                     const int32_t* slots, int64_t rows, int64_t H, int64_t head_dim, int64_t page, int64_t n_pages);
+/* Attention of new tokens over the pages.  Rows q_start[b] .. q_start[b+1] - 1 of q [N, Hq, head_dim] are the last tokens
+ * of request b, which holds lens[b] tokens with them (avsr_paged_plan's lens_out): row i of n sees the keys up to
+ * lens[b] - n + i (causal) or all lens[b] of them.  Query head h reads kv head h / (Hq / Hk).  A row that sees no key
+ * yields zeros; rows behind q_start[B] are left as they were; a key that a row does not see has no influence on it,
+ * whatever it holds; a table entry that names no page hides its keys.  Softmax statistics and sums in fp32; bf16 rounds
+ * the probabilities to bf16 for the second product.  max_q, max_k: at most so many new tokens and keys in any request;
+ * they choose the grid, larger requests still come out right.  Results do not depend on the workspace's contents. */
+int64_t avsr_paged_attn_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim, int64_t max_q,
+                                        int64_t max_k);
+int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, int64_t ldq, int64_t q_head, const void* k_pages,
+                    int64_t k_page_stride, int64_t k_head_stride, const void* v_pages, int64_t v_page_stride,
+                    int64_t v_head_stride, const int32_t* table, int64_t ld_table, int64_t width, const int32_t* lens,
+                    const int32_t* q_start, void* o, int64_t ldo, int64_t o_head, int64_t N, int64_t B, int64_t Hq,
+                    int64_t Hk, int64_t head_dim, int64_t page, int64_t n_pages, int64_t max_q, int64_t max_k,
+                    float scale, int causal, void* workspace, int64_t workspace_bytes);
+/* avsr_embed_tokens for the rows of such a step: positions[row] in place of past + row % T.  A position outside
+ * [0, n_pos) adds nothing and sets *bad_id_flag as a bad id does. */
+int avsr_embed_tokens_at(avsr_stream_t stream, int table_dtype, const int64_t* ids, const void* table, const float* pos,
+                         const int32_t* positions, float* out, int64_t rows, int64_t D, int64_t V, int64_t n_pos,
+                         float scale, int* bad_id_flag);
+/* y[m,n] = act(sum_k x[m,k] * w[n,k] + bias[n]) + residual[m,n] with w[n,k] = (nibble - 8) * scale[n, k / group], the
+ * decoder's nn.Linear layers (hf:277-281,374-376) on 4-bit weights.  packed: 32-bit words of eight nibbles,
+ * word[n/16][k/128][k/8 % 4][n % 16][k/32 % 4], the nibble of k % 8 = e at bit 4*(e/2) + 16*(e%2); scales: bf16
+ * [n/16][k/group][n % 16]; both padded to whole tiles of 16 rows and 128 columns with nibble 8 and scale 0.
+ * group: 32, 64 or 128.  x fp32 or bf16, y and residual fp32 or bf16 (residual of y's type, may be y itself); act NONE,
+ * GELU or RELU.  fp32 sums.  A row of x with a value that is not finite yields NaN. */
+int avsr_w4_matmul(avsr_stream_t stream, int x_dtype, int out_dtype, const void* x, int64_t ldx, const void* packed,
+                   const void* scales, int64_t group, const float* bias, int act, const void* residual, int64_t ldr,
+                   void* y, int64_t ldy, int64_t M, int64_t N, int64_t K);
+
 #ifdef __cplusplus
 }
 #endif

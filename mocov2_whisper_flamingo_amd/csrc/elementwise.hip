@@ -266,7 +266,8 @@ static inline unsigned grid_for(long n, int per_block, long cap) {
 template <typename TW>
 __global__ __launch_bounds__(256) void embed_tokens_kernel(const long* __restrict__ ids, const TW* __restrict__ table,
                                                            const float* __restrict__ pos, float* __restrict__ out, long rows,
-                                                           int T, int past, int D, long V, float scale, int* __restrict__ bad) {
+                                                           int T, int past, int D, long V, float scale, int* __restrict__ bad,
+                                                           const int* __restrict__ positions, long n_pos) {
     const int d4 = D >> 2;
     const long n = rows * d4, stride = (long)gridDim.x * blockDim.x;
     for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += stride) {
@@ -278,7 +279,10 @@ __global__ __launch_bounds__(256) void embed_tokens_kernel(const long* __restric
 #pragma unroll
             for (int k = 0; k < 4; ++k) e[k] = to_f32<TW>(table[id * D + c + k]);
         } else if (c == 0 && bad) atomicOr(bad, 1);
-        const f32x4 pp = *(const f32x4*)(pos + (long)(past + (int)(row % T)) * D + c);
+        f32x4 pp = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (!positions) pp = *(const f32x4*)(pos + (long)(past + (int)(row % T)) * D + c);
+        else if (positions[row] >= 0 && positions[row] < n_pos) pp = *(const f32x4*)(pos + (long)positions[row] * D + c);
+        else if (c == 0 && bad) atomicOr(bad, 1);
         f32x4 o;
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[k] = e[k] * scale + pp[k];
@@ -454,10 +458,27 @@ extern "C" int avsr_embed_tokens(avsr_stream_t stream, int table_dtype, const in
     dim3 grid(grid_for(rows * (D / 4), 256, 4096)), block(256);
     if (table_dtype == AVSR_F32)
         hipLaunchKernelGGL(embed_tokens_kernel<float>, grid, block, 0, s, (const long*)ids, (const float*)table, pos, out,
-                           (long)rows, (int)T, (int)past, (int)D, (long)V, scale, bad_id_flag);
+                           (long)rows, (int)T, (int)past, (int)D, (long)V, scale, bad_id_flag, nullptr, 0);
     else if (table_dtype == AVSR_BF16)
         hipLaunchKernelGGL(embed_tokens_kernel<bf16_t>, grid, block, 0, s, (const long*)ids, (const bf16_t*)table, pos, out,
-                           (long)rows, (int)T, (int)past, (int)D, (long)V, scale, bad_id_flag);
+                           (long)rows, (int)T, (int)past, (int)D, (long)V, scale, bad_id_flag, nullptr, 0);
+    else return AVSR_EINVAL;
+    return avsr_launch_status();
+}
+
+extern "C" int avsr_embed_tokens_at(avsr_stream_t stream, int table_dtype, const int64_t* ids, const void* table, const float* pos,
+                                    const int32_t* positions, float* out, int64_t rows, int64_t D, int64_t V, int64_t n_pos,
+                                    float scale, int* bad_id_flag) {
+    if (!ids || !table || !pos || !positions || !out || rows <= 0 || D <= 0 || V <= 0 || n_pos <= 0) return AVSR_EINVAL;
+    if (D % 4 || ((uintptr_t)table | (uintptr_t)pos | (uintptr_t)out) % 16) return AVSR_EUNSUPPORTED;
+    hipStream_t s = (hipStream_t)stream;
+    dim3 grid(grid_for(rows * (D / 4), 256, 4096)), block(256);
+    if (table_dtype == AVSR_F32)
+        hipLaunchKernelGGL(embed_tokens_kernel<float>, grid, block, 0, s, (const long*)ids, (const float*)table, pos, out,
+                           (long)rows, 1, 0, (int)D, (long)V, scale, bad_id_flag, positions, (long)n_pos);
+    else if (table_dtype == AVSR_BF16)
+        hipLaunchKernelGGL(embed_tokens_kernel<bf16_t>, grid, block, 0, s, (const long*)ids, (const bf16_t*)table, pos, out,
+                           (long)rows, 1, 0, (int)D, (long)V, scale, bad_id_flag, positions, (long)n_pos);
     else return AVSR_EINVAL;
     return avsr_launch_status();
 }

@@ -5,6 +5,8 @@ the stream.
 """
 import ctypes
 import os
+from collections import namedtuple
+
 import torch
 
 from . import _lib
@@ -968,6 +970,235 @@ def embed_tokens(ids, table, pos, past=0, scale=1.0):
                                 B * T, T, past, D, V, pos.shape[0], scale, bad.data_ptr()), "avsr_embed_tokens")
     if int(bad.item()):
         raise IndexError("token id out of range for the embedding table")
+    return out
+
+
+def embed_tokens_at(ids, table, pos, positions, scale=1.0, bad=None):
+    """ids [N] int64, positions [N] int32 -> fp32 [N, D]: table[ids] * scale + pos[positions], for rows of requests of
+    different lengths (``PagedPlan.positions``).  ``bad``: one-element int32 GPU tensor that is set to 1 by an id or position
+    outside its table (whose row then lacks it); without one the call waits for the GPU and raises IndexError."""
+    lib = _lib.load()
+    if ids.dtype != torch.int64 or ids.dim() != 1 or positions.dtype != torch.int32 or positions.shape != ids.shape:
+        raise ValueError("ids must be int64 [N] and positions int32 [N]")
+    if not (table.is_contiguous() and pos.is_contiguous()) or pos.dtype != torch.float32 or table.shape[1:] != pos.shape[1:]:
+        raise ValueError("the tables must be contiguous [V, D] and fp32 [n_pos, D]")
+    _same_gpu(ids, table, pos, positions, bad)
+    V, D = table.shape
+    out = torch.empty((ids.numel(), D), dtype=torch.float32, device=ids.device)
+    if ids.numel() == 0:
+        return out
+    flag = torch.zeros(1, dtype=torch.int32, device=ids.device) if bad is None else bad
+    if flag.dtype != torch.int32 or flag.numel() != 1:
+        raise ValueError("bad must be a one-element int32 tensor")
+    ids, positions = ids.contiguous(), positions.contiguous()
+    check(lib.avsr_embed_tokens_at(_stream(), _dt(table), ids.data_ptr(), table.data_ptr(), pos.data_ptr(), positions.data_ptr(),
+                                   out.data_ptr(), ids.numel(), D, V, pos.shape[0], scale, flag.data_ptr()), "avsr_embed_tokens_at")
+    if bad is None and int(flag.item()):
+        raise IndexError("token id or position out of range for the embedding tables")
+    return out
+
+
+# ---- paged key / value cache and 4-bit weights: serving the decoder ---------------------------------------------------
+PAGE_SIZES = (16, 32, 64, 128, 256)
+PagedPlan = namedtuple("PagedPlan", "q_start slots positions status")
+
+
+def _same_gpu(*ts):
+    """Every tensor on the current device: the launch goes to that device's stream."""
+    _need_cuda(*ts)
+    for t in ts:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise ValueError(f"tensor on {t.device} while cuda:{torch.cuda.current_device()} is the current device")
+
+
+def _ints(t, shape, what):
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)}")
+
+
+def _table(t):
+    if t.dtype != torch.int32 or t.dim() != 2 or 0 in t.shape or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        raise ValueError("the block table must be int32 [requests, pages of a request] with unit inner stride")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _pages(k_pages, v_pages):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError("k_pages and v_pages must be [pages, heads, page, head_dim] of one type")
+    n, H, page, D = k_pages.shape
+    if page not in PAGE_SIZES or D not in (64, 128) or n == 0 or H == 0:
+        raise ValueError(f"page size {page} (one of {PAGE_SIZES}) or head_dim {D} (64 or 128) not supported")
+    for t in (k_pages, v_pages):
+        if t.stride(3) != 1 or t.stride(2) != D:
+            raise ValueError("the [page, head_dim] block of a page and head must be contiguous")
+    return n, H, page, D
+
+
+def paged_plan(lens, new, table, ring, pool, page_size, max_tokens, *, lens_out=None, pool_out=None):
+    """Block tables and slot map of one step for B requests, on the GPU (``avsr_paged_plan``; the header has the rules).
+
+    ``lens`` int32 [B]: tokens each request holds; ``new`` int32 [B]: tokens it adds, or a negative number: it ends and its pages
+    go back.  ``table`` int32 [B, W], ``ring`` int32 [pages] and ``pool`` int32 [2] = {head, count} are the cache's state; the
+    table and the ring are updated in place, the lengths and the pool too unless ``lens_out`` / ``pool_out`` are given.
+    Returns ``PagedPlan(q_start [B+1], slots [max_tokens], positions [max_tokens], status [1])``, int32 on the GPU; status is 0, or
+    says why the step does not fit - then nothing was changed, and the slots are all -1."""
+    lib = _lib.load()
+    lens_out = lens if lens_out is None else lens_out
+    pool_out = pool if pool_out is None else pool_out
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page size must be one of {PAGE_SIZES}")
+    max_tokens = int(max_tokens)
+    if lens.dim() != 1 or lens.numel() == 0 or max_tokens < 1 or ring.dim() != 1 or ring.numel() == 0:
+        raise ValueError("paged_plan needs at least one request, one page and max_tokens >= 1")
+    B, ld = lens.numel(), _table(table)
+    for t, what in ((lens, "lens"), (new, "new"), (lens_out, "lens_out")):
+        _ints(t, (B,), what)
+    _ints(ring, ring.shape, "ring")
+    _ints(pool, (2,), "pool")
+    _ints(pool_out, (2,), "pool_out")
+    if table.shape[0] != B:
+        raise ValueError("the block table needs a row per request")
+    _same_gpu(lens, new, table, ring, pool, lens_out, pool_out)
+    buf = torch.empty(B + 2 + 2 * max_tokens, dtype=torch.int32, device=lens.device)
+    plan = PagedPlan(buf[1:B + 2], buf[B + 2:B + 2 + max_tokens], buf[B + 2 + max_tokens:], buf[:1])
+    ws_bytes = int(lib.avsr_paged_plan_workspace_bytes(B, max_tokens))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=lens.device) if ws_bytes else None
+    check(lib.avsr_paged_plan(_stream(), lens.data_ptr(), new.data_ptr(), table.data_ptr(), ld, table.shape[1], ring.data_ptr(),
+                              ring.numel(), pool.data_ptr(), B, page_size, max_tokens, lens_out.data_ptr(), pool_out.data_ptr(),
+                              plan.q_start.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.status.data_ptr(),
+                              _p(ws)), "avsr_paged_plan")
+    return plan
+
+
+def paged_write(k, v, k_pages, v_pages, slots):
+    """k, v [N, H, D] (rows and heads of any stride) into the pages [pages, H, page, D] at ``slots`` int32 [N] =
+    page * page_size + place (``PagedPlan.slots``); a row with a negative slot is left out, the others are distinct.  fp32 rows are
+    rounded into bf16 pages."""
+    lib = _lib.load()
+    n, H, page, D = _pages(k_pages, v_pages)
+    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (H, D) or k.dtype != v.dtype:
+        raise ValueError(f"k and v must be [N, {H}, {D}] of one type")
+    if k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("k and v need unit inner stride")
+    if _dt(k) == BF16 and _dt(k_pages) == F32:
+        raise TypeError("bf16 rows do not go into fp32 pages")
+    _ints(slots, k.shape[:1], "slots")
+    _same_gpu(k, v, k_pages, v_pages, slots)
+    if k.shape[0] == 0:
+        return
+    check(lib.avsr_paged_write(_stream(), _dt(k), _dt(k_pages), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+                               v.stride(1), k_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1), v_pages.data_ptr(),
+                               v_pages.stride(0), v_pages.stride(1), slots.data_ptr(), k.shape[0], H, D, page, n), "avsr_paged_write")
+
+
+def paged_attn(q, k_pages, v_pages, table, lens, q_start, *, max_q=None, max_k=None, scale=1.0, causal=True, out=None):
+    """Attention of the new tokens q [N, Hq, D] of B requests over their pages (``avsr_paged_attn``).  Rows q_start[b] ..
+    q_start[b+1]-1 are the last tokens of request b, ``lens`` [B] counts its tokens with them; ``causal=False``: each row sees all
+    of them (cross-attention).  Hq is a multiple of the pages' heads.  ``max_q`` / ``max_k``: at most so many new tokens / keys in a
+    request - they choose how the work is split, no result depends on them.  Rows behind the last request are left as they are."""
+    lib = _lib.load()
+    n, Hk, page, D = _pages(k_pages, v_pages)
+    if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hk or q.dtype != k_pages.dtype or q.stride(2) != 1:
+        raise ValueError(f"q must be [N, a multiple of {Hk}, {D}] of the pages' type with unit inner stride")
+    ld, B = _table(table), table.shape[0]
+    _ints(lens, (B,), "lens")
+    _ints(q_start, (B + 1,), "q_start")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+        raise ValueError("out must have q's shape and type, and unit inner stride")
+    N, Hq = q.shape[:2]
+    max_q = N if max_q is None else int(max_q)
+    max_k = table.shape[1] * page if max_k is None else int(max_k)
+    if (N and max_q < 1) or max_k < 1:
+        raise ValueError("max_q and max_k must be positive")
+    _same_gpu(q, k_pages, v_pages, table, lens, q_start, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if N == 0:
+        return out
+    max_q, max_k = min(N, max_q), min(table.shape[1] * page, max_k)
+    ws_bytes = int(lib.avsr_paged_attn_workspace_bytes(N, B, Hq, Hk, D, max_q, max_k))
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    check(lib.avsr_paged_attn(_stream(), _dt(q), q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), k_pages.stride(0),
+                              k_pages.stride(1), v_pages.data_ptr(), v_pages.stride(0), v_pages.stride(1), table.data_ptr(), ld,
+                              table.shape[1], lens.data_ptr(), q_start.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), N, B,
+                              Hq, Hk, D, page, n, max_q, max_k, scale, int(causal), _p(ws), ws_bytes), "avsr_paged_attn")
+    return out
+
+
+W4Weight = namedtuple("W4Weight", "packed scales N K group")
+W4_GROUPS = (32, 64, 128)
+
+
+def w4_pack(q, scales, group):
+    """4-bit weights laid out for :func:`w4_matmul`, once: q [N, K] whole numbers in -8 .. 7, scales [N, ceil(K / group)]
+    (kept in bf16); w[n, k] = q[n, k] * scales[n, k // group]."""
+    if group not in W4_GROUPS:
+        raise ValueError(f"group must be one of {W4_GROUPS}")
+    if q.dim() != 2 or 0 in q.shape or q.dtype.is_floating_point or tuple(scales.shape) != (q.shape[0], -(-q.shape[1] // group)):
+        raise ValueError("w4_pack expects whole numbers [N, K] and scales [N, ceil(K / group)]")
+    if int(q.min()) < -8 or int(q.max()) > 7:
+        raise ValueError("4-bit weights lie in -8 .. 7")
+    N, K = q.shape
+    T, C = -(-N // 16), -(-K // 128)
+    full = torch.zeros((T * 16, C * 128), dtype=torch.int32, device=q.device)
+    full[:N, :K] = q
+    # n = 16 t + i, k = 128 c + 32 s + 8 g + e -> word [t][c][g][i][s], nibble e
+    e = (full + 8).view(T, 16, C, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)
+    place = torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=torch.int32, device=q.device)
+    packed = torch.bitwise_left_shift(e, place).sum(-1).to(torch.int32).contiguous()
+    sc = torch.zeros((T * 16, C * 128 // group), dtype=torch.bfloat16, device=q.device)
+    sc[:N, :scales.shape[1]] = scales
+    return W4Weight(packed, sc.view(T, 16, -1).permute(0, 2, 1).contiguous(), N, K, group)
+
+
+def w4_quantize(weight, group=64):
+    """The nearest 4-bit form of a [N, K] weight: per row and group of columns the scale that takes the largest magnitude to
+    7, rounded to bf16, and every weight to the nearest multiple of it."""
+    if group not in W4_GROUPS:
+        raise ValueError(f"group must be one of {W4_GROUPS}")
+    if weight.dim() != 2 or 0 in weight.shape or not weight.dtype.is_floating_point:
+        raise ValueError("w4_quantize expects a floating-point [N, K] weight")
+    w = weight.detach().float()
+    N, K = w.shape
+    G = -(-K // group)
+    w = torch.nn.functional.pad(w, (0, G * group - K)).view(N, G, group)
+    scales = (w.abs().amax(-1) / 7).to(torch.bfloat16)
+    s = scales.float()[..., None]
+    q = torch.where(s > 0, w / s, torch.zeros_like(w)).round().clamp(-8, 7)
+    return w4_pack(q.view(N, G * group)[:, :K].to(torch.int32), scales, group)
+
+
+def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=None):
+    """act(x @ w^T + bias) + residual for x [M, K] (fp32 or bf16) and a ``W4Weight``: [M, N] of ``out_dtype`` (x's type).
+    ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself."""
+    lib = _lib.load()
+    N, K, group = w.N, w.K, w.group
+    T, C = -(-N // 16), -(-K // 128)
+    if (group not in W4_GROUPS or w.packed.dtype != torch.int32 or w.packed.numel() != T * C * 256 or w.scales.dtype != torch.bfloat16
+            or w.scales.numel() != T * 16 * (C * 128 // group) or not w.packed.is_contiguous() or not w.scales.is_contiguous()):
+        raise ValueError("not a W4Weight of its N, K and group (see w4_pack)")
+    if x.dim() != 2 or x.shape[1] != K or x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < K):
+        raise ValueError(f"x must be [M, {K}] with unit inner stride")
+    M = x.shape[0]
+    odt = out_dtype if out_dtype is not None else (out.dtype if out is not None else x.dtype)
+    if odt not in _DT:
+        raise TypeError(f"unsupported dtype {odt}")
+    for t, what in ((out, "out"), (residual, "residual")):
+        if t is not None and (t.dtype != odt or tuple(t.shape) != (M, N) or t.stride(1) != 1 or (M > 1 and t.stride(0) < N)):
+            raise ValueError(f"{what} must be a row-major [{M}, {N}] tensor of type {odt}")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
+        raise ValueError("bias must be contiguous fp32 [N]")
+    if act not in (ACT_NONE, ACT_GELU, ACT_RELU):
+        raise ValueError("act must be ACT_NONE, ACT_GELU or ACT_RELU")
+    _same_gpu(x, w.packed, w.scales, bias, residual, out)
+    if out is None:
+        out = torch.empty((M, N), dtype=odt, device=x.device)
+    if M == 0:
+        return out
+    row = lambda t: t.stride(0) if M > 1 else t.shape[1]
+    check(lib.avsr_w4_matmul(_stream(), _dt(x), _DT[odt], x.data_ptr(), row(x), w.packed.data_ptr(), w.scales.data_ptr(), group, _p(bias),
+                             act, _p(residual), 0 if residual is None else row(residual), out.data_ptr(), row(out), M, N, K),
+          "avsr_w4_matmul")
     return out
 
 
