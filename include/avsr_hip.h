@@ -558,7 +558,7 @@ int avsr_adamw_step_dev(avsr_stream_t stream, float* param, float* grad, float* 
  * than max_tokens), 8 (a negative length, or a pool that cannot be), and then tables, ring, lengths and pool stay as
  * they are, q_start is all 0 and slots all -1, so that what follows in the step does nothing.  lens_out may be lens and
  * pool_out may be pool.  Workspace: avsr_paged_plan_workspace_bytes (0: none). */
-int64_t avsr_paged_plan_workspace_bytes(int64_t B, int64_t max_tokens);
+int64_t avsr_paged_plan_workspace_bytes(int64_t B, int64_t max_tokens, int64_t n_pages);
 int avsr_paged_plan(avsr_stream_t stream, const int32_t* lens, const int32_t* add, int32_t* table, int64_t ld_table,
                     int64_t width, int32_t* ring, int64_t n_pages, const int32_t* pool, int64_t B, int64_t page,
                     int64_t max_tokens, int32_t* lens_out, int32_t* pool_out, int32_t* q_start, int32_t* slots,
@@ -577,8 +577,8 @@ int avsr_paged_write(avsr_stream_t stream, int in_dtype, int page_dtype, const v
  * whatever it holds; a table entry that names no page hides its keys.  Softmax statistics and sums in fp32; bf16 rounds
  * the probabilities to bf16 for the second product.  max_q, max_k: at most so many new tokens and keys in any request;
  * they choose the grid, larger requests still come out right.  Results do not depend on the workspace's contents. */
-int64_t avsr_paged_attn_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim, int64_t max_q,
-                                        int64_t max_k);
+int64_t avsr_paged_attn_workspace_bytes(int dtype, int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim,
+                                        int64_t max_q, int64_t max_k);
 int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, int64_t ldq, int64_t q_head, const void* k_pages,
                     int64_t k_page_stride, int64_t k_head_stride, const void* v_pages, int64_t v_page_stride,
                     int64_t v_head_stride, const int32_t* table, int64_t ld_table, int64_t width, const int32_t* lens,

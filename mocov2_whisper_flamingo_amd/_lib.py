@@ -133,11 +133,11 @@ SIGNATURES = {
     "avsr_adamw_step": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _f32, _f32, _f32, _f32, _f32, _i64, _vp, _i32]),
     "avsr_step_params": (_i32, [_vp, _vp, _u64, _f32, _f32, _f32, _i64]),
     "avsr_adamw_step_dev": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _f32, _f32, _f32, _f32, _vp, _i32, _vp]),
-    "avsr_paged_plan_workspace_bytes": (_i64, [_i64, _i64]),
+    "avsr_paged_plan_workspace_bytes": (_i64, [_i64, _i64, _i64]),
     "avsr_paged_plan": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "avsr_paged_write": (_i32, [_vp, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
                                 _i64, _i64, _i64, _i64, _i64]),
-    "avsr_paged_attn_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "avsr_paged_attn_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "avsr_paged_attn": (_i32, [_vp, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp, _i64]),
     "avsr_embed_tokens_at": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _f32, _vp]),

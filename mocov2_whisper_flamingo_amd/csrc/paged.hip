@@ -1,189 +1,213 @@
 // Serving a decoder from a paged key / value cache.
 //
-//  * paged_plan_*: block tables, slot map and positions of one step from the requests' lengths, on the GPU.
+//  * paged_plan_*_kernel: block tables, slot map and positions of one step from the requests' lengths, on the GPU.
 //  * paged_write_kernel: the step's new keys and values into their slots.
 //  * paged_attn_few_kernel / paged_attn_chunk_kernel: attention of the new tokens over the pages.
 //
 // A page holds `page` tokens of one layer: element (p, h, t, d) of the keys lives at K + p*sp + h*sh + t*D + d, the
 // values in the same way (the [page, D] block of a page and head is contiguous, page and head strides are free).
 #include "common.h"
+#include <type_traits>
 
 #define LOG2E 1.4426950408889634f
 
 // ================================================================= plan ====
 // Exclusive sums over the requests of {pages taken, pages given back, new tokens} decide everything: request b takes
 // the pages ring[(head + take_b + k) % n], k < need_b, gives its own to ring[(head + count + give_b + k) % n], and its
-// new tokens are rows start_b .. of the step.  The sums are a dependency of all output, so ONE workgroup makes them
-// (1024 requests per pass); what follows is independent per token and page.  Up to PLAN_ONE tokens the same workgroup
-// writes it (one launch: latency is all there is), above that a second launch spreads it over the chip.
+// new tokens are rows start_b .. of the step.  All output depends on the sums, so ONE workgroup makes them; what
+// follows is independent per token and page.  A step of up to PLAN_THREADS requests and PLAN_ONE rows is latency only:
+// the same workgroup writes it, a thread the tokens of its own request where there are one or two, a wave those of a
+// longer prompt.  Above that the sums are made in passes and a second launch spreads the rows over the chip.
 #define PLAN_THREADS 1024
 #define PLAN_ONE 8192
+#define PLAN_BIG (1 << 20)     // largest pool of the one-launch form: 1024 requests of no more pages each do not overflow, one with more fails
 
 struct PlanArgs {
     const int* lens; const int* add; int* table; long ld_table; int width; int* ring; int n_pages; const int* pool;
     int* lens_out; int* pool_out; int B; int shift; int max_tokens; int* q_start; int* slots; int* positions; int* status;
-    int* ws;                       // two-launch form: [3][B] old length, first page taken, first page given; [4] totals
+    int* ws;                       // two-launch form: [3][B] old length, first page taken, first page given; [3] head, count, ok
 };
 
-__device__ __forceinline__ int wave_scan_incl(int v, int lane) {
+// three inclusive scans over the wave
+__device__ __forceinline__ void wave_scan3(int (&v)[3], int lane) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v, o);
-        if (lane >= o) v += u;
+        int u[3];
+#pragma unroll
+        for (int q = 0; q < 3; ++q) u[q] = __shfl_up(v[q], o);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) v[q] += lane >= o ? u[q] : 0;
     }
-    return v;
 }
 
-// what request b asks for; bad: what cannot be
-__device__ __forceinline__ void plan_request(const PlanArgs& a, int b, int& len, int& need, int& give, int& more, int& bad) {
-    len = need = give = more = 0;
+// what request b asks for: v = {pages it takes, pages it gives back, new tokens}; bad: what cannot be
+__device__ __forceinline__ void plan_request(const PlanArgs& a, int b, int& len, int& add, int (&v)[3], int& bad) {
+    len = add = v[0] = v[1] = v[2] = 0;
     if (b >= a.B) return;
     len = a.lens[b];
-    const int add = a.add[b];
-    const long room = (long)a.width << a.shift;
-    if (len < 0) { bad |= 8; len = 0; return; }
-    if (len > room) { bad |= 2; return; }
-    const int have = (len + (1 << a.shift) - 1) >> a.shift;           // len <= room: no overflow near 2^31 (width * page < 2^31)
-    if (add < 0) { give = have; return; }
-    if ((long)len + add > room) { bad |= 2; return; }
-    more = add;
-    need = (int)(((long)len + add + (1 << a.shift) - 1) >> a.shift) - have;
+    add = a.add[b];
+    const long room = (long)a.width << a.shift;                        // < 2^31
+    if (len < 0) { bad |= 8; return; }
+    if (len > room || (add >= 0 && (long)len + add > room)) { bad |= 2; return; }
+    const int up = (1 << a.shift) - 1, have = (int)(((long)len + up) >> a.shift);
+    if (add < 0) { v[1] = have; return; }
+    v[2] = add;
+    v[0] = (int)(((long)len + add + up) >> a.shift) - have;
 }
-
-// Tables, ring and token rows of a step, spread over `nthr` threads of which this is `tid`.  len / take / give / start:
-// per request (start has B + 1); head, count: the ring before the step.
-__device__ void plan_fill(const PlanArgs& a, const int* len, const int* take, const int* give, const int* start, long tid, long nthr,
-                          int head, int count, bool ok) {
-    const int page = 1 << a.shift, total = ok ? start[a.B] : 0;
-    for (long t = tid; t < a.max_tokens; t += nthr) {
-        int slot = -1, pos = 0;
-        if (t < total) {
-            int lo = 0, hi = a.B;                                      // start[lo] <= t < start[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (start[mid] <= t) lo = mid; else hi = mid;
-            }
-            const int n = len[lo], have = (n + page - 1) >> a.shift;
-            pos = n + ((int)t - start[lo]);
-            const int j = pos >> a.shift;
-            int p;
-            if (j < have) p = a.table[lo * a.ld_table + j];
-            else {
-                unsigned at = (unsigned)head + take[lo] + (j - have);
-                p = a.ring[at >= (unsigned)a.n_pages ? at - a.n_pages : at];
-            }
-            slot = (p << a.shift) + (pos & (page - 1));
-        }
-        a.slots[t] = slot;
-        a.positions[t] = pos;
-    }
-    if (!ok) return;
-    const int lane = tid & 63;
-    for (long b = tid >> 6; b < a.B; b += nthr >> 6) {                 // a wave per request
-        const int n = len[b], add = a.add[b], have = (n + page - 1) >> a.shift;
-        int* row = a.table + b * a.ld_table;
-        if (add < 0) {
-            for (int j = lane; j < have; j += 64) {
-                unsigned at = (unsigned)head + count + give[b] + j;    // count + pages given <= n_pages: below 2 n
-                a.ring[at >= (unsigned)a.n_pages ? at - a.n_pages : at] = row[j];
-            }
-        } else {
-            const int need = ((n + add + page - 1) >> a.shift) - have;
-            for (int j = lane; j < need; j += 64) {
-                unsigned at = (unsigned)head + take[b] + j;
-                row[have + j] = a.ring[at >= (unsigned)a.n_pages ? at - a.n_pages : at];
-            }
-        }
-    }
+__device__ __forceinline__ int ring_at(const PlanArgs& a, int head, int k) {          // head + k < 2 n_pages
+    const unsigned at = (unsigned)head + (unsigned)k;
+    return (int)(at >= (unsigned)a.n_pages ? at - a.n_pages : at);
+}
+// token k of a request that held len tokens and takes its new pages from number `take` on
+__device__ __forceinline__ void plan_token(const PlanArgs& a, const int* row, int len, int take, int head, int t, int k) {
+    const int pos = len + k, j = pos >> a.shift, have = (len + (1 << a.shift) - 1) >> a.shift;
+    const int p = j < have ? row[j] : a.ring[ring_at(a, head, take + j - have)];
+    a.slots[t] = (p << a.shift) + (pos & ((1 << a.shift) - 1));
+    a.positions[t] = pos;
+}
+// new table entries, or the ended request's pages into the ring, for j = first, first + step ...
+__device__ __forceinline__ void plan_pages(const PlanArgs& a, int* row, int len, int add, int take, int give, int head, int count, int first, int step) {
+    const int up = (1 << a.shift) - 1, have = (len + up) >> a.shift;
+    if (add < 0)
+        for (int j = first; j < have; j += step) a.ring[ring_at(a, head, count + give + j)] = row[j];
+    else
+        for (int j = have + first; j < (len + add + up) >> a.shift; j += step) row[j] = a.ring[ring_at(a, head, take + j - have)];
 }
 
 template <bool ONE>
-__global__ __launch_bounds__(PLAN_THREADS) void paged_plan_scan_kernel(PlanArgs a) {
+__global__ __launch_bounds__(PLAN_THREADS) void paged_plan_sums_kernel(PlanArgs a) {
     __shared__ int part[3][16];
     __shared__ long red[3][16];
-    __shared__ int s_bad;
-    __shared__ int s_len[ONE ? PLAN_THREADS : 1], s_take[ONE ? PLAN_THREADS : 1], s_give[ONE ? PLAN_THREADS : 1], s_start[ONE ? PLAN_THREADS + 1 : 1];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ int s_bad, s_long;
+    __shared__ int s_list[ONE ? PLAN_THREADS : 1][6];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, waves = blockDim.x >> 6;
     const int head = a.pool[0], count = a.pool[1];
-    if (tid == 0) s_bad = (head < 0 || head >= a.n_pages || count < 0 || count > a.n_pages) ? 8 : 0;
-    __syncthreads();
-    // totals first (nothing is written unless the whole step fits)
-    int bad = 0;
-    long sum[3] = {0, 0, 0};
-    int len, need, give, more;
-    for (int b = tid; b < a.B; b += PLAN_THREADS) {
-        plan_request(a, b, len, need, give, more, bad);
-        sum[0] += need; sum[1] += give; sum[2] += more;
-    }
-    if (bad) atomicOr(&s_bad, bad);
+    int len, add, v[3], bad = (head < 0 || head >= a.n_pages || count < 0 || count > a.n_pages) ? 8 : 0;
+    if (tid == 0) { s_bad = 0; s_long = 0; }
+    int st = 0;
+    if (!ONE) {                                                        // totals first: nothing is written unless the whole step fits
+        long sum[3] = {0, 0, 0};
+        for (int b = tid; b < a.B; b += PLAN_THREADS) {
+            plan_request(a, b, len, add, v, bad);
 #pragma unroll
-    for (int q = 0; q < 3; ++q) {
-        for (int o = 32; o; o >>= 1) sum[q] += __shfl_xor(sum[q], o);
-        if (lane == 0) red[q][w] = sum[q];
-    }
-    __syncthreads();
-    long tot[3] = {0, 0, 0};
+            for (int q = 0; q < 3; ++q) sum[q] += v[q];
+        }
+        __syncthreads();
+        if (bad) atomicOr(&s_bad, bad);
 #pragma unroll
-    for (int q = 0; q < 3; ++q)
-        for (int i = 0; i < PLAN_THREADS / 64; ++i) tot[q] += red[q][i];
-    int st = s_bad;
-    if (tot[0] > count) st |= 1;
-    if (tot[2] > a.max_tokens) st |= 4;
-    if (tot[1] + count > a.n_pages) st |= 8;
-    const bool ok = st == 0;
-    int carry[3] = {0, 0, 0};
+        for (int q = 0; q < 3; ++q) {
+            for (int o = 32; o; o >>= 1) sum[q] += __shfl_xor(sum[q], o);
+            if (lane == 0) red[q][w] = sum[q];
+        }
+        __syncthreads();
+        long tot[3] = {0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            for (int i = 0; i < waves; ++i) tot[q] += red[q][i];
+        st = s_bad | (tot[0] > count ? 1 : 0) | (tot[2] > a.max_tokens ? 4 : 0) | (tot[1] + count > a.n_pages ? 8 : 0);
+    }
+    int carry[3] = {0, 0, 0}, ex[3];
     const int passes = ONE ? 1 : (a.B + PLAN_THREADS - 1) / PLAN_THREADS;
     for (int c = 0; c < passes; ++c) {
         const int b = c * PLAN_THREADS + tid;
-        if (!ONE || c) plan_request(a, b, len, need, give, more, bad);
-        else if (b >= a.B) len = need = give = more = 0;
-        int v[3] = {need, give, more}, in[3];
+        plan_request(a, b, len, add, v, bad);
+        int in[3];
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-            in[q] = wave_scan_incl(ok ? v[q] : 0, lane);
-            if (lane == 63) part[q][w] = in[q];
+            if (ONE) { if (v[q] > PLAN_BIG) bad |= 1 << 30; in[q] = min(v[q], PLAN_BIG); }
+            else in[q] = st ? 0 : v[q];
+            ex[q] = -in[q];
         }
+        wave_scan3(in, lane);
+        if (ONE) {
+            for (int o = 1; o < 64; o <<= 1) bad |= __shfl_xor(bad, o);
+            if (c == 0 && lane == 0) red[0][w] = bad;
+        }
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            if (lane == 63) part[q][w] = in[q];
         __syncthreads();
-        int ex[3];
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
             int base = carry[q], all = 0;
-            for (int i = 0; i < PLAN_THREADS / 64; ++i) {
+            for (int i = 0; i < waves; ++i) {
                 const int u = part[q][i];
-                if (i < w) base += u;
+                base += i < w ? u : 0;
                 all += u;
             }
-            ex[q] = base + in[q] - (ok ? v[q] : 0);
+            ex[q] += base + in[q];
             carry[q] += all;
+        }
+        if (ONE) {
+            for (int i = 0; i < waves; ++i) st |= (int)red[0][i];
+            if (st >> 30) {                                            // a request beyond any pool: the step fails, the status by exact sums
+                long tot[3] = {0, 0, 0};
+                int dummy = 0, l2, a2, v2[3];
+                for (int i = 0; i < a.B; ++i) {
+                    plan_request(a, i, l2, a2, v2, dummy);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) tot[q] += v2[q];
+                }
+                st &= ~(1 << 30);
+                st |= (tot[0] > count ? 1 : 0) | (tot[2] > a.max_tokens ? 4 : 0) | (tot[1] + count > a.n_pages ? 8 : 0);
+            } else st |= (carry[0] > count ? 1 : 0) | (carry[2] > a.max_tokens ? 4 : 0) | ((long)carry[1] + count > a.n_pages ? 8 : 0);
+            if (st) carry[0] = carry[1] = carry[2] = ex[0] = ex[1] = ex[2] = 0;
         }
         if (b < a.B) {
             a.q_start[b] = ex[2];
-            if (ONE) { s_len[tid] = len; s_take[tid] = ex[0]; s_give[tid] = ex[1]; s_start[tid] = ex[2]; }
-            else { a.ws[b] = len; a.ws[a.B + b] = ex[0]; a.ws[2 * (long)a.B + b] = ex[1]; }
-            if (ok) a.lens_out[b] = a.add[b] < 0 ? 0 : len + more;
+            if (!ONE) { a.ws[b] = len; a.ws[a.B + b] = ex[0]; a.ws[2 * (long)a.B + b] = ex[1]; }
+            if (!st) a.lens_out[b] = add < 0 ? 0 : len + add;
             else if (a.lens_out != a.lens) a.lens_out[b] = a.lens[b];
         }
-        __syncthreads();
+        if (!ONE) __syncthreads();
     }
     if (tid == 0) {
         a.q_start[a.B] = carry[2];
-        if (ONE) s_start[a.B] = carry[2];
-        else { int* t = a.ws + 3 * (long)a.B; t[0] = head; t[1] = count; t[2] = ok; }
+        if (!ONE) { int* t = a.ws + 3 * (long)a.B; t[0] = head; t[1] = count; t[2] = !st; }
         a.status[0] = st;
-        if (ok) {
-            unsigned h = (unsigned)head + (unsigned)tot[0];
-            a.pool_out[0] = h >= (unsigned)a.n_pages ? h - a.n_pages : h;
-            a.pool_out[1] = count - (int)tot[0] + (int)tot[1];
+        if (!st) {
+            a.pool_out[0] = ring_at(a, head, carry[0]);
+            a.pool_out[1] = count - carry[0] + carry[1];
         } else if (a.pool_out != a.pool) { a.pool_out[0] = head; a.pool_out[1] = count; }
     }
-    if (ONE) {
-        __syncthreads();
-        plan_fill(a, s_len, s_take, s_give, s_start, tid, PLAN_THREADS, head, count, ok);
+    if (!ONE) return;
+    for (int t = carry[2] + tid; t < a.max_tokens; t += blockDim.x) { a.slots[t] = -1; a.positions[t] = 0; }
+    if (st) return;
+    if (tid < a.B) {
+        int* row = a.table + tid * a.ld_table;
+        if (v[2] <= 2 && v[0] <= 2 && v[1] <= 2) {
+            for (int k = 0; k < v[2]; ++k) plan_token(a, row, len, ex[0], head, ex[2] + k, k);
+            plan_pages(a, row, len, add, ex[0], ex[1], head, count, 0, 1);
+        } else {
+            int* e = s_list[atomicAdd(&s_long, 1)];
+            e[0] = tid; e[1] = len; e[2] = add; e[3] = ex[0]; e[4] = ex[1]; e[5] = ex[2];
+        }
+    }
+    __syncthreads();
+    for (int i = w; i < s_long; i += waves) {
+        const int* e = s_list[i];
+        int* row = a.table + e[0] * a.ld_table;
+        for (int k = lane; k < e[2]; k += 64) plan_token(a, row, e[1], e[3], head, e[5] + k, k);
+        plan_pages(a, row, e[1], e[2], e[3], e[4], head, count, lane, 64);
     }
 }
-__global__ __launch_bounds__(256) void paged_plan_fill_kernel(PlanArgs a) {
-    const int* t = a.ws + 3 * (long)a.B;
-    plan_fill(a, a.ws, a.ws + a.B, a.ws + 2 * (long)a.B, a.q_start, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256, t[0], t[1], t[2]);
+__global__ __launch_bounds__(256) void paged_plan_rows_kernel(PlanArgs a) {
+    const int* s = a.ws + 3 * (long)a.B;
+    const int head = s[0], count = s[1], total = a.q_start[a.B];
+    const long tid = (long)blockIdx.x * 256 + threadIdx.x, nthr = (long)gridDim.x * 256;
+    const int *len = a.ws, *take = a.ws + a.B, *give = a.ws + 2 * (long)a.B;
+    for (long t = tid; t < a.max_tokens; t += nthr) {
+        if (t >= total) { a.slots[t] = -1; a.positions[t] = 0; continue; }
+        int lo = 0, hi = a.B;                                          // q_start[lo] <= t < q_start[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (a.q_start[mid] <= t) lo = mid; else hi = mid;
+        }
+        plan_token(a, a.table + lo * a.ld_table, len[lo], take[lo], head, (int)t, (int)t - a.q_start[lo]);
+    }
+    if (!s[2]) return;
+    for (long b = tid >> 6; b < a.B; b += nthr >> 6)                   // a wave per request
+        plan_pages(a, a.table + b * a.ld_table, len[b], a.add[b], take[b], give[b], head, count, (int)(tid & 63), 64);
 }
 
 static inline int page_shift(int64_t page) {
@@ -191,10 +215,10 @@ static inline int page_shift(int64_t page) {
         if (page == (1 << s)) return s;
     return -1;
 }
-static inline bool plan_one(int64_t B, int64_t max_tokens) { return B <= PLAN_THREADS && max_tokens <= PLAN_ONE; }
+static inline bool plan_one(int64_t B, int64_t max_tokens, int64_t n_pages) { return B <= PLAN_THREADS && max_tokens <= PLAN_ONE && n_pages <= PLAN_BIG; }
 
-extern "C" int64_t avsr_paged_plan_workspace_bytes(int64_t B, int64_t max_tokens) {
-    return plan_one(B, max_tokens) ? 0 : (3 * B + 4) * 4;
+extern "C" int64_t avsr_paged_plan_workspace_bytes(int64_t B, int64_t max_tokens, int64_t n_pages) {
+    return plan_one(B, max_tokens, n_pages) ? 0 : (3 * B + 4) * 4;
 }
 
 extern "C" int avsr_paged_plan(avsr_stream_t stream, const int32_t* lens, const int32_t* add, int32_t* table, int64_t ld_table,
@@ -206,16 +230,20 @@ extern "C" int avsr_paged_plan(avsr_stream_t stream, const int32_t* lens, const 
     const int shift = page_shift(page);
     // slots, lengths and ring positions are 32-bit
     if (shift < 0 || B > (1 << 24) || max_tokens > (1 << 30) || n_pages > (1LL << (30 - shift)) || width > (1LL << (30 - shift))) return AVSR_EUNSUPPORTED;
-    if (!plan_one(B, max_tokens) && !workspace) return AVSR_EINVAL;
+    if (!plan_one(B, max_tokens, n_pages) && !workspace) return AVSR_EINVAL;
     PlanArgs a = {lens, add, table, (long)ld_table, (int)width, ring, (int)n_pages, pool, lens_out, pool_out, (int)B, shift, (int)max_tokens,
                   q_start, slots, positions, status, (int*)workspace};
     hipStream_t s = (hipStream_t)stream;
-    if (plan_one(B, max_tokens)) hipLaunchKernelGGL(paged_plan_scan_kernel<true>, dim3(1), dim3(PLAN_THREADS), 0, s, a);
-    else {
-        hipLaunchKernelGGL(paged_plan_scan_kernel<false>, dim3(1), dim3(PLAN_THREADS), 0, s, a);
+    if (plan_one(B, max_tokens, n_pages)) {
+        // a thread per request, and enough for the rows to be done in a few turns
+        const int64_t want = B > max_tokens / 4 ? B : max_tokens / 4;
+        const int threads = want >= PLAN_THREADS ? PLAN_THREADS : (int)((want + 63) / 64 * 64);
+        hipLaunchKernelGGL(paged_plan_sums_kernel<true>, dim3(1), dim3(threads), 0, s, a);
+    } else {
+        hipLaunchKernelGGL(paged_plan_sums_kernel<false>, dim3(1), dim3(PLAN_THREADS), 0, s, a);
         int64_t blocks = (max_tokens + 255) / 256, more = (B + 3) / 4;
         blocks = blocks > more ? blocks : more;
-        hipLaunchKernelGGL(paged_plan_fill_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(paged_plan_rows_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, s, a);
     }
     return avsr_launch_status();
 }
@@ -319,7 +347,8 @@ struct AttnArgs {
     const int* lens; const int* q_start;
     void* o; long ldo, ho;
     int B, Hk, G, N, shift, n_pages; float c; int causal;     // c = scale * log2(e)
-    int splits, tiles_few, few_rows; float* part;  // few: key splits, row tiles per request; few_rows: largest request it takes (0 = any)
+    int splits, few_rows;                         // key splits; largest request of the first kernel (0 = any)
+    float *part, *part_ml;                        // [rows][splits][D] sums and [rows][splits]{m, l} of a split grid
 };
 
 // Rows, lengths of request b, kept inside what the arrays hold.
@@ -331,6 +360,14 @@ __device__ __forceinline__ Req request(const AttnArgs& a, int b) {
     r.nq = max(min(e, a.N) - r.q0, 0);
     r.len = min(max(a.lens[b], 0), a.width << a.shift);
     return r;
+}
+
+__device__ __forceinline__ bool finite(float f) { return (__builtin_bit_cast(unsigned, f) & 0x7F800000u) != 0x7F800000u; }
+// the halves (bf16) of v whose exponent is all ones - infinities and NaN - cleared; odd: set if there were any
+__device__ __forceinline__ unsigned finite_half(unsigned v, bool& odd) {
+    const bool lo = (v & 0x7F80u) == 0x7F80u, hi = (v & 0x7F800000u) == 0x7F800000u;
+    odd |= lo || hi;
+    return v & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
 }
 
 template <typename T, int D> struct Frag;
@@ -391,13 +428,13 @@ template <int D> struct Frag<bf16_t, D> {
     }
     static __device__ __forceinline__ void zero_key(V& v, int j) { v.x[j] = (vrow_t)(0u); }
     static __device__ __forceinline__ int key_of_v(int j, int g) { return 8 * g + j; }
-    static __device__ __forceinline__ bool odd_value(const V& v) {       // any value that is not finite
-        bool f = false;
+    static __device__ __forceinline__ bool keep_finite(V& v) {           // clears what is not finite; whether there was any
+        bool odd = false;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int w = 0; w < VW / 2; ++w) f |= (v.x[j][w] & 0x7F80u) == 0x7F80u || (v.x[j][w] & 0x7F800000u) == 0x7F800000u;
-        return f;
+            for (int w = 0; w < VW / 2; ++w) v.x[j][w] = finite_half(v.x[j][w], odd);
+        return odd;
     }
     static __device__ __forceinline__ f32x4 pv(const V& v, int e, const f32x4 (&p)[2], f32x4 o) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(column(v, e), probs(p), o, 0, 0, 0);
@@ -451,15 +488,19 @@ template <int D> struct Frag<float, D> {
         for (int w = 0; w < VW / 4; ++w) v.x[j][w] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     static __device__ __forceinline__ int key_of_v(int j, int g) { return 16 * (j >> 2) + 4 * g + (j & 3); }
-    static __device__ __forceinline__ bool odd_value(const V& v) {
-        bool f = false;
+    static __device__ __forceinline__ bool keep_finite(V& v) {
+        bool odd = false;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
             for (int w = 0; w < VW / 4; ++w)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) f |= (__builtin_bit_cast(unsigned, v.x[j][w][x]) & 0x7F800000u) == 0x7F800000u;
-        return f;
+                for (int x = 0; x < 4; ++x) {
+                    const bool bad = !finite(v.x[j][w][x]);
+                    odd |= bad;
+                    v.x[j][w][x] = bad ? 0.f : v.x[j][w][x];
+                }
+        return odd;
     }
     static __device__ __forceinline__ f32x4 pv(const V& v, int e, const f32x4 (&p)[2], f32x4 o) {
 #pragma unroll
@@ -480,12 +521,11 @@ __device__ __forceinline__ float max_over_groups(float v) {
 
 // The pages of tile kt (keys 32 kt ..): uniform over the wave.  An entry that names no page leaves its keys unseen.
 struct TilePages { int p0, p1; };
-__device__ __forceinline__ TilePages tile_pages(const AttnArgs& a, const int* row, int kt, int kend) {
+__device__ __forceinline__ TilePages tile_pages(const AttnArgs& a, const int* row, int kt) {
     TilePages t;
-    const int last = (kend - 1) >> a.shift;                              // kend >= 1
     const int j = (kt * 32) >> a.shift;
-    t.p0 = row[min(j, last)];
-    t.p1 = a.shift == 4 ? row[min(j + 1, last)] : t.p0;
+    t.p0 = row[min(j, a.width - 1)];
+    t.p1 = a.shift == 4 ? row[min(j + 1, a.width - 1)] : t.p0;
     return t;
 }
 template <typename F, typename T>
@@ -516,45 +556,45 @@ template <int NT, int D> struct State {
 };
 
 // One tile of 32 keys into the state.  limit[n]: the last key the lane's row of tile n sees; kmin / kmax: the smallest /
-// largest of them over the wave's rows (a tile that ends at or before kmin needs no comparison).
+// largest of them over the wave's rows (a tile that ends at or before kmin needs no comparison).  In a tile that some row
+// sees in part, values behind every row's last key are cleared, and ones that are not finite (0 * inf for a row that does
+// not see them) are left out of the product and added to the rows that do.
 template <typename F, int NT, int D>
 __device__ __forceinline__ void attend_tile(State<NT, D>& st, const typename F::Q (&q)[NT], const typename F::K& k, typename F::V& v,
-                                            const int (&limit)[NT], int kt, int kmin, int kmax, bool pages_ok, TilePages tp,
-                                            const AttnArgs& a, int lane) {
+                                            const int (&limit)[NT], int hk, int kt, int kmin, int kmax, TilePages tp, const AttnArgs& a, int lane) {
+    typedef typename F::T T;
     const int g = lane >> 4, k0 = kt * 32;
-    const bool whole = pages_ok && k0 + 31 <= kmin;
+    const bool bad0 = (unsigned)tp.p0 >= (unsigned)a.n_pages, bad1 = (unsigned)tp.p1 >= (unsigned)a.n_pages;
+    const bool whole = !bad0 && !bad1 && k0 + 31 <= kmin;
     bool odd = false;
-    if (!whole) {                                     // nothing a key beyond every row holds may reach the products
-        const bool bad0 = (unsigned)tp.p0 >= (unsigned)a.n_pages, bad1 = (unsigned)tp.p1 >= (unsigned)a.n_pages;
+    if (!whole) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int key = F::key_of_v(j, g);
             if (k0 + key > kmax || ((key & 16) ? bad1 : bad0)) F::zero_key(v, j);
         }
-        odd = __ballot(F::odd_value(v)) != 0;          // 0 * inf: a row's unseen keys need care
+        odd = __any(F::keep_finite(v));
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         f32x4 s[2];
         F::scores(s, k, q[n]);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[t][r] *= a.c;
         if (!whole) {
-            const bool bad0 = (unsigned)tp.p0 >= (unsigned)a.n_pages, bad1 = (unsigned)tp.p1 >= (unsigned)a.n_pages;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int key = F::key_of_score(t, r, g);
-                    s[t][r] = (k0 + key > limit[n] || ((key & 16) ? bad1 : bad0)) ? -INFINITY : s[t][r] * a.c;
+                    if (k0 + key > limit[n] || ((key & 16) ? bad1 : bad0)) s[t][r] = -INFINITY;
                 }
-        } else {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) s[t][r] *= a.c;
         }
         float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         mx = fmaxf(st.m[n], max_over_groups(mx));
-        if (__ballot(mx > st.m[n])) {                  // some row's maximum moved
+        if (__any(mx > st.m[n])) {                     // some row's maximum moved
             const float al = mx == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st.m[n] - mx);
             st.m[n] = mx;
             st.l[n] *= al;
@@ -571,53 +611,64 @@ __device__ __forceinline__ void attend_tile(State<NT, D>& st, const typename F::
                 sum += s[t][r];
             }
         st.l[n] += sum;
-        if (!odd) {
 #pragma unroll
-            for (int e = 0; e < D / 16; ++e) st.o[n][e] = F::pv(v, e, s, st.o[n][e]);
-        } else {                                       // row by row, its unseen keys' values out of the product
-            for (int r = 0; r < 16; ++r) {
-                const int lim = __builtin_amdgcn_readlane(limit[n], r);
-                typename F::V vr = v;
+        for (int e = 0; e < D / 16; ++e) st.o[n][e] = F::pv(v, e, s, st.o[n][e]);
+    }
+    if (odd) {
+#pragma unroll 1
+        for (int key = 0; key < 32; ++key) {
+            if (k0 + key > kmax || ((key & 16) && a.shift == 4 ? bad1 : bad0)) continue;
+            const long page = (key & 16) && a.shift == 4 ? tp.p1 : tp.p0;
+            const T* p = (const T*)a.v + page * a.svp + hk * a.svh + (long)((k0 + key) & ((1 << a.shift) - 1)) * D + (D / 4) * g;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (k0 + F::key_of_v(j, g) > lim) F::zero_key(vr, j);
+            for (int r = 0; r < 4; ++r)
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e) {
-                    const f32x4 x = F::pv(vr, e, s, st.o[n][e]);
+                    const float f = to_f32<T>(p[(D / 16) * r + e]);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) st.o[n][e][y] = (lane & 15) == r ? x[y] : st.o[n][e][y];
+                    for (int n = 0; n < NT; ++n) st.o[n][e][r] += !finite(f) && k0 + key <= limit[n] ? f : 0.f;
                 }
-            }
         }
     }
 }
 
-// Tiles first, first + step, ... < end of the request's keys.  The next tile's keys and values are in flight while a
-// tile is computed, its page numbers one tile further ahead.
-template <typename F, typename T, int NT, int D>
+// Tiles first, first + step, ... < end of the request's keys.  AHEAD: the next tile's keys and values are in flight while a
+// tile is computed, its page numbers one tile further ahead; without, other waves' tiles are.  `loaded`: tile `first` is
+// already on its way.
+template <typename F> struct Stage { typename F::K k; typename F::V v; TilePages tp; };
+template <typename F, typename T, int NT, int D, bool AHEAD>
 __device__ __forceinline__ void attend(State<NT, D>& st, const AttnArgs& a, const typename F::Q (&q)[NT], const int (&limit)[NT],
-                                       const int* row, int hk, int first, int step, int end, int kmin, int kmax, int lane) {
+                                       const int* row, int hk, int first, int step, int end, int kmin, int kmax, int lane,
+                                       Stage<F> (&sg)[AHEAD ? 2 : 1], bool loaded) {
     if (first >= end) return;
     const int i = lane & 15, g = lane >> 4;
-    typename F::K k[2];
-    typename F::V v[2];
-    TilePages tp[2], next;
-    tp[0] = tile_pages(a, row, first, kmax + 1);
-    load_tile<F, T>(a, k[0], v[0], tp[0], first, hk, i, g, D);
-    next = tile_pages(a, row, min(first + step, end - 1), kmax + 1);
-    auto one = [&](int kt, int cur) {
-        if (kt + step < end) {
-            tp[cur ^ 1] = next;
-            load_tile<F, T>(a, k[cur ^ 1], v[cur ^ 1], next, kt + step, hk, i, g, D);
-            next = tile_pages(a, row, min(kt + 2 * step, end - 1), kmax + 1);
-        }
-        const TilePages p = tp[cur];
-        const bool ok = (unsigned)p.p0 < (unsigned)a.n_pages && (unsigned)p.p1 < (unsigned)a.n_pages;
-        attend_tile<F, NT, D>(st, q, k[cur], v[cur], limit, kt, kmin, kmax, ok, p, a, lane);
+    if (!loaded) {
+        sg[0].tp = tile_pages(a, row, first);
+        load_tile<F, T>(a, sg[0].k, sg[0].v, sg[0].tp, first, hk, i, g, D);
+    }
+    TilePages next = tile_pages(a, row, first + step);
+    auto compute = [&](int kt, Stage<F>& s) {
+        attend_tile<F, NT, D>(st, q, s.k, s.v, limit, hk, kt, kmin, kmax, s.tp, a, lane);
     };
-    for (int kt = first; kt < end; kt += 2 * step) {
-        one(kt, 0);
-        if (kt + step < end) one(kt + step, 1);
+    auto fetch = [&](int kt, Stage<F>& s) {
+        s.tp = next;
+        load_tile<F, T>(a, s.k, s.v, next, kt, hk, i, g, D);
+        next = tile_pages(a, row, kt + step);
+    };
+    if constexpr (AHEAD) {
+        for (int kt = first; kt < end; kt += 2 * step) {
+            if (kt + step < end) fetch(kt + step, sg[1]);
+            compute(kt, sg[0]);
+            if (kt + step < end) {
+                if (kt + 2 * step < end) fetch(kt + 2 * step, sg[0]);
+                compute(kt + step, sg[1]);
+            }
+        }
+    } else {
+        for (int kt = first; kt < end; kt += step) {
+            compute(kt, sg[0]);
+            if (kt + step < end) fetch(kt + step, sg[0]);
+        }
     }
 }
 
@@ -635,22 +686,31 @@ template <int D> __device__ __forceinline__ void store_vals(float* p, const floa
     for (int c = 0; c < D / 16; ++c) *(f32x4*)(p + 4 * c) = *(const f32x4*)(x + 4 * c);
 }
 
-// ---- few rows: the four waves of a workgroup take every fourth tile of the keys and are merged through LDS; a split
-// grid leaves {m, l, O} per row and split for paged_attn_join_kernel.
-#define FEW_WAVES 4
-template <typename T, int D>
-__global__ __launch_bounds__(64 * FEW_WAVES) void paged_attn_few_kernel(AttnArgs a) {
+// ---- few rows: the WAVES waves of a workgroup take the tiles of the keys in turn and are merged through LDS; a split
+// grid leaves {m, l} and O of every row and split to paged_attn_join_kernel.
+#ifndef FEW_OCC
+#define FEW_OCC (sizeof(T) * D <= 256 ? 3 : 2)
+#endif
+template <typename T, int D, int WAVES, bool AHEAD>
+__global__ __launch_bounds__(64 * WAVES, FEW_OCC) void paged_attn_few_kernel(AttnArgs a) {
     typedef Frag<T, D> F;
-    __shared__ float s_m[FEW_WAVES][16], s_l[FEW_WAVES][16];
-    __shared__ float s_o[FEW_WAVES][16][D + 4];
+    __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+    __shared__ float s_o[WAVES][16][D + 4];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int split = blockIdx.x % a.splits, x = blockIdx.x / a.splits;
     const int hk = x % a.Hk, b = x / a.Hk;
+    const int* row = a.table + b * a.ld_table;
+    Stage<F> sg[AHEAD ? 2 : 1];
+    // the first tile does not depend on the request's length: it is under way while that is read
+    bool loaded = AHEAD && a.splits == 1 && (w * 32) >> a.shift < a.width;
+    if (loaded) {
+        sg[0].tp = tile_pages(a, row, w);
+        load_tile<F, T>(a, sg[0].k, sg[0].v, sg[0].tp, w, hk, i, g, D);
+    }
     const Req r = request(a, b);
     const int rows = r.nq * a.G;
     if (a.few_rows && rows > a.few_rows) return;
-    const int* row = a.table + b * a.ld_table;
     for (int r0 = blockIdx.y * 16; r0 < rows; r0 += gridDim.y * 16) {
         const int n_rows = min(16, rows - r0);
         const int tok0 = r0 / a.G, tok1 = (r0 + n_rows - 1) / a.G;
@@ -664,7 +724,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_attn_few_kernel(AttnArgs
         st.clear();
         const int tiles = kmax >= 0 ? (kmax >> 5) + 1 : 0;
         const int per = (tiles + a.splits - 1) / a.splits, t0 = split * per, t1 = min(tiles, t0 + per);
-        if (kmax >= 0) attend<F, T, 1, D>(st, a, q, limit, row, hk, t0 + w, FEW_WAVES, t1, kmin, kmax, lane);
+        attend<F, T, 1, D, AHEAD>(st, a, q, limit, row, hk, t0 + w, WAVES, t1, kmin, kmax, lane, sg, loaded);
+        loaded = false;
         st.l[0] = xor_add<32>(xor_add<16>(st.l[0]));
         if (g == 0) { s_m[w][i] = st.m[0]; s_l[w][i] = st.l[0]; }
         if (i < n_rows) {
@@ -674,40 +735,40 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void paged_attn_few_kernel(AttnArgs
                 for (int e = 0; e < D / 16; ++e) s_o[w][i][(D / 4) * g + (D / 16) * rr + e] = st.o[0][e][rr];
         }
         __syncthreads();
-        // 16 columns a thread
-        for (int c = threadIdx.x; c < n_rows * (D / 16); c += 64 * FEW_WAVES) {
-            const int rw = c / (D / 16), d = (c % (D / 16)) * 16;
+        // 8 columns a thread
+        for (int c = threadIdx.x; c < n_rows * (D / 8); c += 64 * WAVES) {
+            const int rw = c / (D / 8), d = (c % (D / 8)) * 8;
             float m = s_m[0][rw];
 #pragma unroll
-            for (int u = 1; u < FEW_WAVES; ++u) m = fmaxf(m, s_m[u][rw]);
+            for (int u = 1; u < WAVES; ++u) m = fmaxf(m, s_m[u][rw]);
             const float ref = m == -INFINITY ? 0.f : m;
-            float l = 0.f, o[16];
+            float l = 0.f, o[8];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = 0.f;
+            for (int j = 0; j < 8; ++j) o[j] = 0.f;
 #pragma unroll
-            for (int u = 0; u < FEW_WAVES; ++u) {
+            for (int u = 0; u < WAVES; ++u) {
                 const float f = __builtin_amdgcn_exp2f(s_m[u][rw] - ref);
                 l = fmaf(f, s_l[u][rw], l);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = fmaf(f, s_o[u][rw][d + j], o[j]);
+                for (int j = 0; j < 8; ++j) o[j] = fmaf(f, s_o[u][rw][d + j], o[j]);
             }
             const int t = (r0 + rw) / a.G, h = hk * a.G + (r0 + rw) - t * a.G;
             if (a.splits == 1) {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] *= inv;
-                store_vals<64>((T*)a.o + (long)(r.q0 + t) * a.ldo + (long)h * a.ho + d, o);
+                for (int j = 0; j < 8; ++j) o[j] *= inv;
+                store_vals<32>((T*)a.o + (long)(r.q0 + t) * a.ldo + (long)h * a.ho + d, o);
             } else {
-                float* p = a.part + (((long)(r.q0 + t) * (a.Hk * a.G) + h) * a.splits + split) * (D + 4);
-                store_vals<64>(p + 4 + d, o);
-                if (d == 0) { p[0] = m; p[1] = l; }
+                const long y = ((long)(r.q0 + t) * (a.Hk * a.G) + h) * a.splits + split;
+                store_vals<32>(a.part + y * D + d, o);
+                if (d == 0) *(f32x2*)(a.part_ml + y * 2) = (f32x2){m, l};
             }
         }
         __syncthreads();
     }
 }
 
-// Joins the splits of a row: a wave per row, one or two columns a lane.
+// Joins the splits of a row, a wave per row: lane s weighs split s, then every lane adds up its columns.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
     const int lane = threadIdx.x & 63;
@@ -715,52 +776,75 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
     const long x = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (x >= rows) return;
     const int t = (int)(x / H), h = (int)(x - t * H);
-    // rows that no request of the few kernel owns were not written there: nothing of theirs is read or stored here
-    int lo = 0, hi = a.B;
-    if (t < a.q_start[0] || t >= a.q_start[a.B]) return;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.q_start[mid] <= t) lo = mid; else hi = mid;
-    }
-    const Req r = request(a, lo);
-    if (t < r.q0 || t >= r.q0 + r.nq || (a.few_rows && r.nq * a.G > a.few_rows)) return;
-    const float* p = a.part + x * a.splits * (D + 4);
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, p[s * (D + 4)]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[D / 64];
+    if (t < a.q_start[0] || t >= a.q_start[a.B]) return;       // rows of no request were not written, and stay as they are
+    const f32x2 ml = lane < a.splits ? *(const f32x2*)(a.part_ml + (x * a.splits + lane) * 2) : (f32x2){-INFINITY, 0.f};
+    const float m = wave_max(ml[0]);
+    float w = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m);
+    const float l = wave_sum(w * ml[1]);
+    w *= l == 0.f ? 0.f : 1.f / l;
+    const float* p = a.part + x * a.splits * D + lane * (D / 64);
+    float o[D / 64];
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) o[c] = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        const float* ps = p + s * (D + 4);
-        const float f = __builtin_amdgcn_exp2f(ps[0] - ref);
-        l = fmaf(f, ps[1], l);
+    for (int s0 = 0; s0 < a.splits; s0 += 8) {                 // eight loads in flight; lanes behind the last split weigh 0
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) o[c] = fmaf(f, ps[4 + 64 * c + lane], o[c]);
+        for (int u = 0; u < 8; ++u) {
+            const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s0 + u));
+            const float* ps = p + (long)min(s0 + u, a.splits - 1) * D;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) o[c] = fmaf(f, ps[c], o[c]);
+        }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* out = (T*)a.o + (long)t * a.ldo + (long)h * a.ho;
+    T* out = (T*)a.o + (long)t * a.ldo + (long)h * a.ho + lane * (D / 64);
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) out[64 * c + lane] = from_f32<T>(o[c] * inv);
+    for (int c = 0; c < D / 64; ++c) out[c] = from_f32<T>(o[c]);
 }
 
-// ---- many rows: each of the four waves takes 16 NT rows of the tile and walks all of its keys.
+// ---- many rows.  The row tiles of all requests (TR rows each) are dealt out with the longest request's first, so that the
+// last workgroups to start are short ones: their work goes with the number of keys.  The order is found by every workgroup
+// for itself, a lane per request; with more than 64 requests, tiles are numbered in the requests' order, request b's from
+// q_start[b]*G/TR + b on (one more than it can fill, so that no sum is needed).
+struct RowTile { Req r; int b, rows, r0; };
+template <int TR> __device__ __forceinline__ RowTile row_tile(const AttnArgs& a, int tile, int lane) {
+    RowTile t;
+    int start;
+    if (a.B <= 64) {
+        Req r = {0, 0, 0};
+        if (lane < a.B) r = request(a, lane);
+        const int mine = r.nq * a.G > a.few_rows ? (r.nq * a.G + TR - 1) / TR : 0;
+        int before = 0;
+        for (int j = 0; j < a.B; ++j) {
+            const int len = __builtin_amdgcn_readlane(r.len, j), n = __builtin_amdgcn_readlane(mine, j);
+            before += len > r.len || (len == r.len && j < lane) ? n : 0;
+        }
+        const unsigned long long who = __ballot(tile >= before && tile < before + mine);
+        t.b = who ? __builtin_ctzll(who) : 0;
+        start = who ? __builtin_amdgcn_readlane(before, t.b) : 1 << 30;      // no such tile
+    } else {
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((int)((long)a.q_start[mid] * a.G / TR) + mid <= tile) lo = mid; else hi = mid;
+        }
+        t.b = lo;
+        start = (int)((long)a.q_start[lo] * a.G / TR) + lo;
+    }
+    t.r = request(a, t.b);
+    t.rows = t.r.nq * a.G;
+    t.r0 = start > tile ? -(1 << 30) : (tile - start) * TR;
+    if (a.causal && t.r0 >= 0) t.r0 = ((t.rows + TR - 1) / TR - 1) * TR - t.r0;     // the last rows see the most
+    return t;
+}
+// fp32: each of the four waves takes 16 NT rows of the tile and walks its keys, straight from the pages.
 template <typename T, int D, int NT>
-__global__ __launch_bounds__(256) void paged_attn_chunk_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnArgs a) {
     typedef Frag<T, D> F;
-    constexpr int TR = 64 * NT;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % a.Hk, tile = blockIdx.x / a.Hk;
-    // request b owns the tiles from q_start[b]*G/TR + b on: at least one more than it fills
-    int lo = 0, hi = a.B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if ((int)((long)a.q_start[mid] * a.G / TR) + mid <= tile) lo = mid; else hi = mid;
-    }
-    const Req r = request(a, lo);
-    const int rows = r.nq * a.G;
-    const int r0 = (tile - ((int)((long)a.q_start[lo] * a.G / TR) + lo)) * TR + w * 16 * NT;
+    const int hk = blockIdx.x % a.Hk, split = blockIdx.x / a.Hk % a.splits, tile = blockIdx.x / a.Hk / a.splits;
+    const RowTile rt = row_tile<64 * NT>(a, tile, lane);
+    const Req r = rt.r;
+    const int rows = rt.rows, r0 = rt.r0 + w * 16 * NT;
     if (rows <= a.few_rows || r0 < 0 || r0 >= rows) return;
     const int n_rows = min(16 * NT, rows - r0);
     const int base = a.causal ? r.len - r.nq : r.len - 1;
@@ -776,11 +860,13 @@ __global__ __launch_bounds__(256) void paged_attn_chunk_kernel(AttnArgs a) {
     }
     State<NT, D> st;
     st.clear();
-    if (kmax >= 0) attend<F, T, NT, D>(st, a, q, limit, a.table + lo * a.ld_table, hk, 0, 1, (kmax >> 5) + 1, kmin, kmax, lane);
+    const int tiles = kmax >= 0 ? (kmax >> 5) + 1 : 0, per = (tiles + a.splits - 1) / a.splits, t0 = split * per;
+    Stage<F> sg[2];
+    attend<F, T, NT, D, true>(st, a, q, limit, a.table + rt.b * a.ld_table, hk, t0, 1, min(tiles, t0 + per), kmin, kmax, lane, sg, false);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const float l = xor_add<32>(xor_add<16>(st.l[n]));
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = a.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
         if (16 * n + i >= n_rows) continue;
         const int my = r0 + 16 * n + i, tok = my / a.G, head = hk * a.G + my - tok * a.G;
         float o[D / 4];
@@ -788,52 +874,355 @@ __global__ __launch_bounds__(256) void paged_attn_chunk_kernel(AttnArgs a) {
         for (int rr = 0; rr < 4; ++rr)
 #pragma unroll
             for (int e = 0; e < D / 16; ++e) o[(D / 16) * rr + e] = st.o[n][e][rr] * inv;
-        store_vals<D>((T*)a.o + (long)(r.q0 + tok) * a.ldo + (long)head * a.ho + (D / 4) * g, o);
+        if (a.splits == 1) store_vals<D>((T*)a.o + (long)(r.q0 + tok) * a.ldo + (long)head * a.ho + (D / 4) * g, o);
+        else {
+            const long x = ((long)(r.q0 + tok) * (a.Hk * a.G) + head) * a.splits + split;
+            store_vals<D>(a.part + x * D + (D / 4) * g, o);
+            if (g == 0) *(f32x2*)(a.part_ml + x * 2) = (f32x2){st.m[n], l};
+        }
+    }
+}
+
+// bf16: tiles of 64 keys go to LDS once for the workgroup's four waves (LDS-DMA, two buffers, one barrier per tile), and
+// a wave keeps RT tiles of 32 rows, so that a fragment read from LDS feeds RT matrix instructions.  S^T and O^T as
+// above on v_mfma_f32_32x32x16_bf16 (A row / B column lane & 31, k = 8 (lane / 32) + j; C column lane & 31, row
+// (i & 3) + 8 (i >> 2) + 4 (lane / 32)); V fragments come transposed out of LDS.  Per score the vector unit has a
+// maximum, a multiply-add, an exponential, an addition and half a conversion to do, more cycles than the matrix pipe
+// needs for the two products of a 64-column head: the maximum is only compared (the reference point moves when a score
+// exceeds it by 2^8), the scale's sign is taken into Q so that raw scores can be compared.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+template <int D> struct KvTile {
+    static constexpr int CH = D / 8;                                  // 16-byte chunks of a key row
+    static constexpr int PIECES = 16 * CH / 64;                       // DMA instructions of 16 keys
+    // chunk c of a row stands at c ^ swizzle(row), so that neither fragment read below hits a bank twice
+    static __device__ __forceinline__ int kswz(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
+    static __device__ __forceinline__ int vswz(int row) { return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
+    // A fragment is read at a lane's offset (bytes, one per 16 or 32 columns, the same for every run of 32 keys) plus a constant.
+    // Keys: row lane & 31, columns 16 ks + 8 (lane / 32) ..
+    static __device__ __forceinline__ int koff(int ks, int lane) {
+        const int row = lane & 31;
+        return (row * D + (((2 * ks + (lane >> 5)) ^ kswz(row)) << 3)) * 2;
+    }
+    static __device__ __forceinline__ bf16x8 kfrag(const char* K, int off) { return *(const bf16x8*)(K + off); }
+    // Values, transposed: columns 32 db + (lane & 31) of the keys 16 s2 + {0..3, 8..11} + 4 (lane / 32), the order of a score register's
+    // keys.  16 lanes read four 32-byte pieces of four rows; which is a swizzle's bits do not depend on s2.
+    static __device__ __forceinline__ int voff(int db, int lane) {
+        const int i16 = lane & 15, row = 4 * (lane >> 5) + (i16 >> 2), col = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+        return (row * D + (((col >> 3) ^ vswz(row)) << 3) + (col & 7)) * 2;
+    }
+    static __device__ __forceinline__ bf16x8 vfrag(const char* V, int s2, int off) {
+        bf16x8 f;
+#pragma unroll
+        for (int jh = 0; jh < 2; ++jh) {
+            const char* p = V + off + (16 * s2 + 8 * jh) * D * 2;
+            const bf16x4 t = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) f[4 * jh + x] = t[x];
+        }
+        return f;
+    }
+};
+
+// keys of half a dword each behind `last` cleared out of a V fragment (keys k0 + 16 s2 + ...)
+__device__ __forceinline__ u32x4 cut_keys(u32x4 v, int first, int hf, int last) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        const int key = first + 8 * (x >> 1) + 4 * hf + 2 * (x & 1);
+        v[x] &= (key <= last ? 0xFFFFu : 0u) | (key + 1 <= last ? 0xFFFF0000u : 0u);
+    }
+    return v;
+}
+__device__ __forceinline__ u32x4 finite_part(u32x4 v, bool& odd) {
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[x] = finite_half(v[x], odd);
+    return v;
+}
+
+#ifndef CHUNK_UNROLL
+#define CHUNK_UNROLL 2
+#endif
+#ifndef CHUNK_NBUF
+#define CHUNK_NBUF (D == 64 ? 3 : 2)
+#endif
+#ifndef CHUNK_OCC
+#define CHUNK_OCC (D == 64 ? 3 : 2)
+#endif
+template <int D, int RT>
+__global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnArgs a) {
+    typedef KvTile<D> L;
+    typedef bf16_t T;
+    constexpr int NBUF = CHUNK_NBUF;
+    __shared__ __attribute__((aligned(16))) bf16_t Ks[NBUF][64 * D], Vs[NBUF][64 * D];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int r32 = lane & 31, hf = lane >> 5;
+    const int hk = blockIdx.x % a.Hk, split = blockIdx.x / a.Hk % a.splits, tile = blockIdx.x / a.Hk / a.splits;
+    const RowTile rt = row_tile<128 * RT>(a, tile, lane);
+    const Req r = rt.r;
+    if (rt.rows <= a.few_rows || rt.r0 < 0 || rt.r0 >= rt.rows) return;
+    const int wg_rows = min(128 * RT, rt.rows - rt.r0);
+    const int base = a.causal ? r.len - r.nq : r.len - 1;
+    const int kmax_wg = a.causal ? base + (rt.r0 + wg_rows - 1) / a.G : base;      // the last key of the workgroup's rows
+    // this wave's rows; a wave without any helps to move the tiles
+    const int r0 = rt.r0 + w * 32 * RT, n_rows = max(0, min(32 * RT, rt.rows - r0));
+    const int kmin = n_rows == 0 ? -1 : a.causal ? base + r0 / a.G : base;
+    const int kmax = n_rows == 0 ? -1 : a.causal ? base + (r0 + n_rows - 1) / a.G : base;
+    bf16x8 q[RT][D / 16];
+    int limit[RT];
+    const unsigned flip = a.c < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+        const bool ok = 32 * n + r32 < n_rows;
+        const int my = ok ? r0 + 32 * n + r32 : 0, tok = my / a.G, head = hk * a.G + my - tok * a.G;
+        const T* p = (const T*)a.q + (long)(r.q0 + tok) * a.ldq + (long)head * a.hq + 8 * hf;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            u32x4 v = {0u, 0u, 0u, 0u};
+            if (ok) v = *(const u32x4*)(p + 16 * ks);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] ^= flip;
+            q[n][ks] = __builtin_bit_cast(bf16x8, v);
+        }
+        limit[n] = ok ? (a.causal ? base + tok : base) : -1;
+    }
+    const float c = fmaxf(fabsf(a.c), 1e-37f);                     // never 0: -inf times it stays -inf
+    const float lazy = 8.f / c;
+    f32x16 o[RT][D / 32];
+    float m[RT], nm[RT], thr[RT], l[RT];
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+        m[n] = thr[n] = -INFINITY; nm[n] = l[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[n][d][x] = 0.f;
+    }
+    const int tiles = kmax_wg >= 0 ? (kmax_wg >> 6) + 1 : 0, per = (tiles + a.splits - 1) / a.splits;
+    const int t0 = split * per, t1 = min(tiles, t0 + per);
+    const int* row = a.table + rt.b * a.ld_table;
+    // 64 entries of the block table, a lane each, from entry `first` on: a scalar would have to be fetched anew for every
+    // tile behind the DMA's back, and its wait would be one for the DMA
+    int first = t0 * 64 >> a.shift;
+    int entries = t0 < t1 ? row[min(first + lane, a.width - 1)] : 0;
+    unsigned kmove[L::PIECES], vmove[L::PIECES];
+#pragma unroll
+    for (int u = 0; u < L::PIECES; ++u) {
+        const int lr = (64 / L::CH) * u + lane / L::CH, ch = lane & (L::CH - 1), rw = 16 * w + lr;
+        kmove[u] = (lr * D + ((ch ^ L::kswz(rw)) << 3)) * 2;
+        vmove[u] = (lr * D + ((ch ^ L::vswz(rw)) << 3)) * 2;
+    }
+    int kr[D / 16], vr[D / 32];
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) kr[ks] = L::koff(ks, lane);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) vr[d] = L::voff(d, lane);
+    unsigned pages = 0;                                    // a nibble per tile in flight, the oldest lowest: which runs' pages exist
+    // Tile kt into buffer buf; wave w moves run w of its four runs of 16 keys, of the keys and of the values.
+    auto move = [&](int kt, int buf, int age) {
+        if (((kt * 64 + 48) >> a.shift) - first >= 64) {
+            first = kt * 64 >> a.shift;
+            entries = row[min(first + lane, a.width - 1)];
+        }
+        int p[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) p[u] = __builtin_amdgcn_readlane(entries, ((kt * 64 + 16 * u) >> a.shift) - first);
+        const int pw = __builtin_amdgcn_readlane(entries, ((kt * 64 + 16 * w) >> a.shift) - first);
+        const long page = (unsigned)pw < (unsigned)a.n_pages ? pw : 0;
+        const int in = (kt * 64 + 16 * w) & ((1 << a.shift) - 1);
+        const char* k = (const char*)((const T*)a.k + page * a.sp + hk * a.sh + in * D);
+        const char* v = (const char*)((const T*)a.v + page * a.svp + hk * a.svh + in * D);
+#pragma unroll
+        for (int u = 0; u < L::PIECES; ++u) {
+            dma_piece(k, kmove[u], (const char*)&Ks[buf][(16 * w) * D + u * 512]);
+            dma_piece(v, vmove[u], (const char*)&Vs[buf][(16 * w) * D + u * 512]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) pages |= ((unsigned)p[u] < (unsigned)a.n_pages ? 1u : 0u) << (4 * age + u);
+    };
+    if (t0 < t1) {
+#pragma unroll
+        for (int u = 0; u < NBUF - 1; ++u)
+            if (t0 + u < t1) move(t0 + u, u, u);
+    }
+    for (int kt = t0, buf = 0; kt < t1; ++kt, buf = buf == NBUF - 1 ? 0 : buf + 1) {
+        // this wave's part of the tile is in LDS (a younger tile may still be on its way) ...
+        if (NBUF == 3 && kt + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L::PIECES) : "memory");
+        else if (NBUF == 4 && kt + 2 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * L::PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                                          // ... and everyone's, and the buffer before it is free
+        const unsigned have = pages & 15u;
+        pages >>= 4;
+        if (kt + NBUF - 1 < t1) move(kt + NBUF - 1, buf == 0 ? NBUF - 1 : buf - 1, NBUF - 2);
+        if (kt * 64 > kmax) continue;                             // none of this wave's rows sees the tile
+        auto half = [&](int st, auto whole_tile) {                // 32 of the tile's keys
+            constexpr bool whole = decltype(whole_tile)::value;
+            const char *K = (const char*)Ks[buf] + st * 64 * D, *V = (const char*)Vs[buf] + st * 64 * D;
+            const int k0 = kt * 64 + 32 * st;
+            const bool ok0 = have >> (2 * st) & 1, ok1 = have >> (2 * st + 1) & 1;
+            f32x16 s[RT];
+            bf16x8 kf[D / 16];
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) kf[ks] = L::kfrag(K, kr[ks]);
+#pragma unroll
+            for (int n = 0; n < RT; ++n) {
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[n][x] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], q[n][ks], s[n], 0, 0, 0);
+            }
+            bf16x8 p[RT][2];
+#pragma unroll
+            for (int n = 0; n < RT; ++n) {
+                if constexpr (!whole) {
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int key = (x & 3) + 8 * (x >> 2) + 4 * hf;
+                        if (k0 + key > limit[n] || !(x < 8 ? ok0 : ok1)) s[n][x] = -INFINITY;
+                    }
+                }
+                float mx = max3(s[n][0], s[n][1], s[n][2]), my = max3(s[n][3], s[n][4], s[n][5]);
+                mx = max3(mx, s[n][6], s[n][7]); my = max3(my, s[n][8], s[n][9]);
+                mx = max3(mx, s[n][10], s[n][11]); my = max3(my, s[n][12], s[n][13]);
+                mx = max3(mx, s[n][14], s[n][15]);
+                mx = max3(mx, my, my);
+                if (__any(mx > thr[n])) {                         // rare after the first tiles
+                    const unsigned u = __builtin_bit_cast(unsigned, mx);
+                    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+                    const float top = fmaxf(m[n], fmaxf(__builtin_bit_cast(float, (unsigned)sw[0]), __builtin_bit_cast(float, (unsigned)sw[1])));
+                    const float al = top > m[n] ? __builtin_amdgcn_exp2f((m[n] - top) * c) : 1.f;
+                    m[n] = top;
+                    thr[n] = top + lazy;
+                    nm[n] = top == -INFINITY ? 0.f : -(top * c);
+                    l[n] *= al;
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) o[n][d][x] *= al;
+                }
+                float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                for (int x = 0; x < 16; x += 2) {
+                    s[n][x] = __builtin_amdgcn_exp2f(fmaf(s[n][x], c, nm[n]));
+                    s[n][x + 1] = __builtin_amdgcn_exp2f(fmaf(s[n][x + 1], c, nm[n]));
+                    s0 += s[n][x];
+                    s1 += s[n][x + 1];
+                }
+                l[n] += s0 + s1;
+                // rounding to bf16 for the product: half a step of 2^-8 relative per probability; the sum l is of the unrounded ones
+#pragma unroll
+                for (int x = 0; x < 8; ++x) { p[n][0][x] = (bf16_t)s[n][x]; p[n][1][x] = (bf16_t)s[n][8 + x]; }
+            }
+            // In a tile that some row sees in part, values behind every row's last key are cleared, and ones that are not
+            // finite (0 * inf for a row that does not see them) are added to the rows that do.
+            bool odd = false;
+#pragma unroll
+            for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                for (int d = 0; d < D / 32; ++d) {
+                    bf16x8 vf = L::vfrag(V, s2, vr[d]);
+                    if constexpr (!whole) vf = __builtin_bit_cast(bf16x8, finite_part(cut_keys(__builtin_bit_cast(u32x4, vf), k0 + 16 * s2, hf, (s2 ? ok1 : ok0) ? kmax : -1), odd));
+#pragma unroll
+                    for (int n = 0; n < RT; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[n][s2], o[n][d], 0, 0, 0);
+                }
+            if (!whole && __any(odd)) {
+#pragma unroll 1
+                for (int key = 0; key < 32; ++key)
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const int col = 32 * d + 8 * y + 4 * hf;
+                            const bf16x4 v = *(const bf16x4*)(V + (key * D + (((col >> 3) ^ L::vswz(key)) << 3) + (col & 7)) * 2);
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) {
+                                const float f = (float)v[z];
+#pragma unroll
+                                for (int n = 0; n < RT; ++n) o[n][d][4 * y + z] += !finite(f) && k0 + key <= limit[n] && (key < 16 ? ok0 : ok1) ? f : 0.f;
+                            }
+                        }
+            }
+        };
+        if (kt * 64 + 63 <= kmin && have == 15u) {                // every row sees all of it
+#pragma unroll CHUNK_UNROLL
+            for (int st = 0; st < 2; ++st) half(st, std::true_type{});
+        } else {
+#pragma unroll 1
+            for (int st = 0; st < 2; ++st) half(st, std::false_type{});
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < RT; ++n) {
+        const float sum = xor_add<32>(l[n]);
+        const float inv = a.splits > 1 ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+        if (32 * n + r32 >= n_rows) continue;
+        const int my = r0 + 32 * n + r32, tok = my / a.G, head = hk * a.G + my - tok * a.G;
+        const long x = ((long)(r.q0 + tok) * (a.Hk * a.G) + head) * a.splits + split;
+        T* out = (T*)a.o + (long)(r.q0 + tok) * a.ldo + (long)head * a.ho;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                f32x4 v;
+                bf16x4 b;
+#pragma unroll
+                for (int z = 0; z < 4; ++z) { v[z] = o[n][d][4 * y + z] * inv; b[z] = (bf16_t)v[z]; }
+                if (a.splits == 1) *(bf16x4*)(out + 32 * d + 8 * y + 4 * hf) = b;
+                else *(f32x4*)(a.part + x * D + 32 * d + 8 * y + 4 * hf) = v;
+            }
+        if (a.splits > 1 && hf == 0) *(f32x2*)(a.part_ml + x * 2) = (f32x2){m[n] * c, sum};
     }
 }
 
 // Requests of up to FEW_ROWS rows (tokens times the heads that share a kv head) go to the first kernel.
 #define FEW_ROWS 64
-struct AttnPlan { int splits, tiles_few, few_rows; bool few, chunk; long chunk_tiles; };
-static AttnPlan attn_plan(int64_t N, int64_t B, int64_t Hk, int64_t G, int64_t max_q, int64_t max_k, int chunk_rows) {
+#ifndef CHUNK_RT
+#define CHUNK_RT 1
+#endif
+struct AttnPlan { int waves, splits, tiles_few, few_rows, chunk_rows; bool few, chunk; int64_t chunk_tiles, grid_few, grid_chunk, floats; };
+static AttnPlan attn_plan(int dtype, int64_t D, int64_t N, int64_t B, int64_t Hk, int64_t G, int64_t max_q, int64_t max_k) {
     AttnPlan p;
     const int64_t rows = max_q * G;
     p.chunk = rows > FEW_ROWS;
     p.few = !(p.chunk && B == 1 && N * G > FEW_ROWS);          // one large request: nothing for the first kernel
-    p.few_rows = p.chunk ? FEW_ROWS : 0;
+    p.few_rows = p.few && p.chunk ? FEW_ROWS : 0;
     p.tiles_few = (int)((rows < FEW_ROWS ? rows : FEW_ROWS) + 15) / 16;
-    const int64_t wgs = B * Hk * p.tiles_few;
-    int64_t s = (1024 + wgs - 1) / wgs;
-    const int64_t most = (max_k + 255) / 256;
-    s = s < most ? s : most;
+    p.chunk_rows = dtype == AVSR_F32 ? (D == 64 ? 128 : 64) : 128 * CHUNK_RT;
+    p.chunk_tiles = p.chunk ? N * G / p.chunk_rows + B : 0;
+    // Key splits where the row tiles do not fill the chip (256 CUs): the first kernel gets up to 1024 workgroups, of 512 keys
+    // at least; the second up to 512, of 256 keys at least.
+    const int64_t wgs = p.chunk ? Hk * p.chunk_tiles : B * Hk * p.tiles_few;
+    const int64_t fill = (p.chunk ? 512 : 1024) / wgs, most = p.chunk ? (max_k + 255) / 256 : (max_k + 511) / 512;
+    const int64_t s = fill < most ? fill : most;
     p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-    p.chunk_tiles = N * G / chunk_rows + B;
+    p.waves = p.few && wgs * p.splits <= 512 ? 8 : 4;
+    p.grid_few = p.few ? B * Hk * p.splits : 0;
+    p.grid_chunk = Hk * p.chunk_tiles * p.splits;
+    p.floats = p.splits > 1 ? N * Hk * G * p.splits * (D + 2) : 0;
     return p;
 }
-#define CHUNK_NT 2
-extern "C" int64_t avsr_paged_attn_workspace_bytes(int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim, int64_t max_q,
+extern "C" int64_t avsr_paged_attn_workspace_bytes(int dtype, int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim, int64_t max_q,
                                                    int64_t max_k) {
     if (N <= 0 || B <= 0 || Hk <= 0 || Hq % Hk || max_q <= 0 || max_k <= 0) return 0;
-    const AttnPlan p = attn_plan(N, B, Hk, Hq / Hk, max_q, max_k, 64 * CHUNK_NT);
-    return p.few && p.splits > 1 ? N * Hq * p.splits * (head_dim + 4) * 4 : 0;
+    return attn_plan(dtype, head_dim, N, B, Hk, Hq / Hk, max_q, max_k).floats * 4;
 }
 
+#ifndef FEW_AHEAD
+#define FEW_AHEAD (sizeof(T) * D <= 128)
+#endif
 template <typename T, int D>
 static int launch_attn(hipStream_t s, AttnArgs a, const AttnPlan& p) {
-    const int few_rows = p.few_rows;
-    if (p.few) {
-        a.few_rows = few_rows;
-        a.splits = p.splits;
-        hipLaunchKernelGGL((paged_attn_few_kernel<T, D>), dim3((unsigned)((long)a.B * a.Hk * p.splits), p.tiles_few), dim3(64 * FEW_WAVES), 0, s, a);
-        if (p.splits > 1) {
-            const long rows = (long)a.N * a.Hk * a.G;
-            hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-        }
-    }
+    const dim3 few((unsigned)p.grid_few, p.tiles_few);
+    constexpr bool ahead = FEW_AHEAD;
+    if (p.few && p.waves == 4) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 4, ahead>), few, dim3(256), 0, s, a);
+    else if (p.few) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, 8, ahead>), few, dim3(512), 0, s, a);
     if (p.chunk) {
-        a.few_rows = p.few ? few_rows : 0;
-        hipLaunchKernelGGL((paged_attn_chunk_kernel<T, D, CHUNK_NT>), dim3((unsigned)(p.chunk_tiles * a.Hk)), dim3(256), 0, s, a);
+        if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_attn_rows_kernel<T, D, D == 64 ? 2 : 1>), dim3((unsigned)p.grid_chunk), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((paged_attn_chunk_kernel<D, CHUNK_RT>), dim3((unsigned)p.grid_chunk), dim3(256), 0, s, a);
     }
+    if (p.splits > 1) hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.N * a.Hk * a.G + 3) / 4)), dim3(256), 0, s, a);
     return avsr_launch_status();
 }
 
@@ -854,13 +1243,13 @@ extern "C" int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, i
     if (N > (1 << 28) || N * Hq > (1LL << 30) || B > (1 << 24) || B * Hk > (1LL << 24)) return AVSR_EUNSUPPORTED;
     if (N == 0) return AVSR_OK;
     const int64_t mq = max_q < N ? max_q : N, mk = max_k < width * page ? max_k : width * page;
-    const AttnPlan p = attn_plan(N, B, Hk, Hq / Hk, mq, mk, 64 * CHUNK_NT);
-    const int64_t need = p.few && p.splits > 1 ? N * Hq * p.splits * (head_dim + 4) * 4 : 0;
-    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)) return AVSR_EINVAL;
-    if (p.chunk_tiles * Hk > 0x7fffffff) return AVSR_EUNSUPPORTED;
+    const AttnPlan p = attn_plan(dtype, head_dim, N, B, Hk, Hq / Hk, mq, mk);
+    if (p.floats && (!workspace || workspace_bytes < p.floats * 4 || (uintptr_t)workspace % 16)) return AVSR_EINVAL;
+    if (p.grid_few > 0x7fffffff || p.grid_chunk > 0x7ffffff0) return AVSR_EUNSUPPORTED;
+    float* part = (float*)workspace;
     AttnArgs a = {q, ldq, q_head, k_pages, v_pages, k_page_stride, k_head_stride, v_page_stride, v_head_stride, table, ld_table, (int)width,
                   lens, q_start, o, ldo, o_head, (int)B, (int)Hk, (int)(Hq / Hk), (int)N, shift, (int)n_pages, scale * LOG2E, causal != 0,
-                  1, p.tiles_few, p.few_rows, (float*)workspace};
+                  p.splits, p.few_rows, part, part ? part + N * Hq * p.splits * head_dim : nullptr};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == AVSR_BF16) return head_dim == 64 ? launch_attn<bf16_t, 64>(s, a, p) : launch_attn<bf16_t, 128>(s, a, p);
     return head_dim == 64 ? launch_attn<float, 64>(s, a, p) : launch_attn<float, 128>(s, a, p);

@@ -982,7 +982,7 @@ def embed_tokens_at(ids, table, pos, positions, scale=1.0, bad=None):
         raise ValueError("ids must be int64 [N] and positions int32 [N]")
     if not (table.is_contiguous() and pos.is_contiguous()) or pos.dtype != torch.float32 or table.shape[1:] != pos.shape[1:]:
         raise ValueError("the tables must be contiguous [V, D] and fp32 [n_pos, D]")
-    _same_gpu(ids, table, pos, positions, bad)
+    stream = _gpu_stream(ids, table, pos, positions, bad)
     V, D = table.shape
     out = torch.empty((ids.numel(), D), dtype=torch.float32, device=ids.device)
     if ids.numel() == 0:
@@ -991,7 +991,7 @@ def embed_tokens_at(ids, table, pos, positions, scale=1.0, bad=None):
     if flag.dtype != torch.int32 or flag.numel() != 1:
         raise ValueError("bad must be a one-element int32 tensor")
     ids, positions = ids.contiguous(), positions.contiguous()
-    check(lib.avsr_embed_tokens_at(_stream(), _dt(table), ids.data_ptr(), table.data_ptr(), pos.data_ptr(), positions.data_ptr(),
+    check(lib.avsr_embed_tokens_at(stream, _dt(table), ids.data_ptr(), table.data_ptr(), pos.data_ptr(), positions.data_ptr(),
                                    out.data_ptr(), ids.numel(), D, V, pos.shape[0], scale, flag.data_ptr()), "avsr_embed_tokens_at")
     if bad is None and int(flag.item()):
         raise IndexError("token id or position out of range for the embedding tables")
@@ -1003,35 +1003,45 @@ PAGE_SIZES = (16, 32, 64, 128, 256)
 PagedPlan = namedtuple("PagedPlan", "q_start slots positions status")
 
 
-def _same_gpu(*ts):
-    """Every tensor on the current device: the launch goes to that device's stream."""
-    _need_cuda(*ts)
+def _gpu_stream(*ts):
+    """The current stream (raw) of the device that every tensor is on; the launch goes there, so it has to be the current one."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device.index != torch.cuda.current_device():
-            raise ValueError(f"tensor on {t.device} while cuda:{torch.cuda.current_device()} is the current device")
+        if t is not None and t.get_device() != dev or dev < 0:
+            _need_cuda(*ts)
+            raise ValueError("tensors on different devices")
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on cuda:{dev} while cuda:{torch.cuda.current_device()} is the current device")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _ints(t, shape, what):
-    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)}")
+def _ints(t, n, what):
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of {n} values")
 
 
 def _table(t):
-    if t.dtype != torch.int32 or t.dim() != 2 or 0 in t.shape or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if t.dim() != 2:
+        raise ValueError("the block table must be [requests, pages of a request]")
+    (B, W), (ld, one) = t.shape, t.stride()
+    if t.dtype is not torch.int32 or B == 0 or W == 0 or one != 1 or (B > 1 and ld < W):
         raise ValueError("the block table must be int32 [requests, pages of a request] with unit inner stride")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return B, W, ld if B > 1 else W
 
 
 def _pages(k_pages, v_pages):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    """(pages, heads, page, head_dim, page and head strides of keys and values)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or shape != v_pages.shape or k_pages.dtype is not v_pages.dtype:
         raise ValueError("k_pages and v_pages must be [pages, heads, page, head_dim] of one type")
-    n, H, page, D = k_pages.shape
-    if page not in PAGE_SIZES or D not in (64, 128) or n == 0 or H == 0:
+    n, H, page, D = shape
+    if page not in PAGE_SIZES or (D != 64 and D != 128) or n == 0 or H == 0:
         raise ValueError(f"page size {page} (one of {PAGE_SIZES}) or head_dim {D} (64 or 128) not supported")
-    for t in (k_pages, v_pages):
-        if t.stride(3) != 1 or t.stride(2) != D:
-            raise ValueError("the [page, head_dim] block of a page and head must be contiguous")
-    return n, H, page, D
+    kp, kh, kt, k1 = k_pages.stride()
+    vp, vh, vt, v1 = v_pages.stride()
+    if k1 != 1 or v1 != 1 or kt != D or vt != D:
+        raise ValueError("the [page, head_dim] block of a page and head must be contiguous")
+    return n, H, page, D, kp, kh, vp, vh
 
 
 def paged_plan(lens, new, table, ring, pool, page_size, max_tokens, *, lens_out=None, pool_out=None):
@@ -1042,86 +1052,98 @@ def paged_plan(lens, new, table, ring, pool, page_size, max_tokens, *, lens_out=
     table and the ring are updated in place, the lengths and the pool too unless ``lens_out`` / ``pool_out`` are given.
     Returns ``PagedPlan(q_start [B+1], slots [max_tokens], positions [max_tokens], status [1])``, int32 on the GPU; status is 0, or
     says why the step does not fit - then nothing was changed, and the slots are all -1."""
-    lib = _lib.load()
-    lens_out = lens if lens_out is None else lens_out
-    pool_out = pool if pool_out is None else pool_out
+    if lens_out is None:
+        lens_out = lens
+    if pool_out is None:
+        pool_out = pool
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page size must be one of {PAGE_SIZES}")
-    max_tokens = int(max_tokens)
-    if lens.dim() != 1 or lens.numel() == 0 or max_tokens < 1 or ring.dim() != 1 or ring.numel() == 0:
+    max_tokens, B, n = int(max_tokens), lens.numel(), ring.numel()
+    if B == 0 or max_tokens < 1 or n == 0:
         raise ValueError("paged_plan needs at least one request, one page and max_tokens >= 1")
-    B, ld = lens.numel(), _table(table)
-    for t, what in ((lens, "lens"), (new, "new"), (lens_out, "lens_out")):
-        _ints(t, (B,), what)
-    _ints(ring, ring.shape, "ring")
-    _ints(pool, (2,), "pool")
-    _ints(pool_out, (2,), "pool_out")
-    if table.shape[0] != B:
+    rows, width, ld = _table(table)
+    if rows != B:
         raise ValueError("the block table needs a row per request")
-    _same_gpu(lens, new, table, ring, pool, lens_out, pool_out)
+    _ints(lens, B, "lens")
+    _ints(new, B, "new")
+    _ints(lens_out, B, "lens_out")
+    _ints(ring, n, "ring")
+    _ints(pool, 2, "pool")
+    _ints(pool_out, 2, "pool_out")
+    stream = _gpu_stream(lens, new, table, ring, pool, lens_out, pool_out)
+    lib = _lib.load()
     buf = torch.empty(B + 2 + 2 * max_tokens, dtype=torch.int32, device=lens.device)
-    plan = PagedPlan(buf[1:B + 2], buf[B + 2:B + 2 + max_tokens], buf[B + 2 + max_tokens:], buf[:1])
-    ws_bytes = int(lib.avsr_paged_plan_workspace_bytes(B, max_tokens))
+    q_start, slots, positions, status = buf.split_with_sizes((B + 1, max_tokens, max_tokens, 1))
+    at = buf.data_ptr()
+    ws_bytes = lib.avsr_paged_plan_workspace_bytes(B, max_tokens, n)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=lens.device) if ws_bytes else None
-    check(lib.avsr_paged_plan(_stream(), lens.data_ptr(), new.data_ptr(), table.data_ptr(), ld, table.shape[1], ring.data_ptr(),
-                              ring.numel(), pool.data_ptr(), B, page_size, max_tokens, lens_out.data_ptr(), pool_out.data_ptr(),
-                              plan.q_start.data_ptr(), plan.slots.data_ptr(), plan.positions.data_ptr(), plan.status.data_ptr(),
-                              _p(ws)), "avsr_paged_plan")
-    return plan
+    rc = lib.avsr_paged_plan(stream, lens.data_ptr(), new.data_ptr(), table.data_ptr(), ld, width, ring.data_ptr(), n, pool.data_ptr(), B,
+                             page_size, max_tokens, lens_out.data_ptr(), pool_out.data_ptr(), at, at + 4 * (B + 1),
+                             at + 4 * (B + 1 + max_tokens), at + 4 * (B + 1 + 2 * max_tokens), _p(ws))
+    check(rc, "avsr_paged_plan")
+    return PagedPlan(q_start, slots, positions, status)
 
 
 def paged_write(k, v, k_pages, v_pages, slots):
     """k, v [N, H, D] (rows and heads of any stride) into the pages [pages, H, page, D] at ``slots`` int32 [N] =
     page * page_size + place (``PagedPlan.slots``); a row with a negative slot is left out, the others are distinct.  fp32 rows are
     rounded into bf16 pages."""
-    lib = _lib.load()
-    n, H, page, D = _pages(k_pages, v_pages)
-    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (H, D) or k.dtype != v.dtype:
+    n, H, page, D, kp, kh, vp, vh = _pages(k_pages, v_pages)
+    shape = k.shape
+    if len(shape) != 3 or shape != v.shape or shape[1] != H or shape[2] != D or k.dtype is not v.dtype:
         raise ValueError(f"k and v must be [N, {H}, {D}] of one type")
-    if k.stride(2) != 1 or v.stride(2) != 1:
+    N = shape[0]
+    (kt, kr, k1), (vt, vr, v1) = k.stride(), v.stride()
+    if k1 != 1 or v1 != 1:
         raise ValueError("k and v need unit inner stride")
-    if _dt(k) == BF16 and _dt(k_pages) == F32:
+    it, pt = _dt(k), _dt(k_pages)
+    if it == BF16 and pt == F32:
         raise TypeError("bf16 rows do not go into fp32 pages")
-    _ints(slots, k.shape[:1], "slots")
-    _same_gpu(k, v, k_pages, v_pages, slots)
-    if k.shape[0] == 0:
+    _ints(slots, N, "slots")
+    stream = _gpu_stream(k, v, k_pages, v_pages, slots)
+    if N == 0:
         return
-    check(lib.avsr_paged_write(_stream(), _dt(k), _dt(k_pages), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                               v.stride(1), k_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1), v_pages.data_ptr(),
-                               v_pages.stride(0), v_pages.stride(1), slots.data_ptr(), k.shape[0], H, D, page, n), "avsr_paged_write")
+    rc = _lib.load().avsr_paged_write(stream, it, pt, k.data_ptr(), kt, kr, v.data_ptr(), vt, vr, k_pages.data_ptr(), kp, kh,
+                                      v_pages.data_ptr(), vp, vh, slots.data_ptr(), N, H, D, page, n)
+    check(rc, "avsr_paged_write")
 
 
 def paged_attn(q, k_pages, v_pages, table, lens, q_start, *, max_q=None, max_k=None, scale=1.0, causal=True, out=None):
     """Attention of the new tokens q [N, Hq, D] of B requests over their pages (``avsr_paged_attn``).  Rows q_start[b] ..
     q_start[b+1]-1 are the last tokens of request b, ``lens`` [B] counts its tokens with them; ``causal=False``: each row sees all
     of them (cross-attention).  Hq is a multiple of the pages' heads.  ``max_q`` / ``max_k``: at most so many new tokens / keys in a
-    request - they choose how the work is split, no result depends on them.  Rows behind the last request are left as they are."""
-    lib = _lib.load()
-    n, Hk, page, D = _pages(k_pages, v_pages)
-    if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hk or q.dtype != k_pages.dtype or q.stride(2) != 1:
-        raise ValueError(f"q must be [N, a multiple of {Hk}, {D}] of the pages' type with unit inner stride")
-    ld, B = _table(table), table.shape[0]
-    _ints(lens, (B,), "lens")
-    _ints(q_start, (B + 1,), "q_start")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
-        raise ValueError("out must have q's shape and type, and unit inner stride")
-    N, Hq = q.shape[:2]
+    request - they choose how the work is split, larger requests still come out right.  Rows behind the last request are left as
+    they are."""
+    n, Hk, page, D, kp, kh, vp, vh = _pages(k_pages, v_pages)
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != D or shape[1] == 0 or shape[1] % Hk or q.dtype is not k_pages.dtype:
+        raise ValueError(f"q must be [N, a multiple of {Hk}, {D}] of the pages' type")
+    N, Hq, _ = shape
+    qt, qh, q1 = q.stride()
+    B, W, ld = _table(table)
+    _ints(lens, B, "lens")
+    _ints(q_start, B + 1, "q_start")
+    if q1 != 1 or (out is not None and (out.shape != shape or out.dtype is not q.dtype or out.stride(2) != 1)):
+        raise ValueError("q and out need unit inner stride, out q's shape and type")
     max_q = N if max_q is None else int(max_q)
-    max_k = table.shape[1] * page if max_k is None else int(max_k)
+    max_k = W * page if max_k is None else int(max_k)
     if (N and max_q < 1) or max_k < 1:
         raise ValueError("max_q and max_k must be positive")
-    _same_gpu(q, k_pages, v_pages, table, lens, q_start, out)
+    dt = _dt(q)
+    stream = _gpu_stream(q, k_pages, v_pages, table, lens, q_start, out)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
     if N == 0:
         return out
-    max_q, max_k = min(N, max_q), min(table.shape[1] * page, max_k)
-    ws_bytes = int(lib.avsr_paged_attn_workspace_bytes(N, B, Hq, Hk, D, max_q, max_k))
+    lib = _lib.load()
+    max_q, max_k = min(N, max_q), min(W * page, max_k)
+    ws_bytes = lib.avsr_paged_attn_workspace_bytes(dt, N, B, Hq, Hk, D, max_q, max_k)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    check(lib.avsr_paged_attn(_stream(), _dt(q), q.data_ptr(), q.stride(0), q.stride(1), k_pages.data_ptr(), k_pages.stride(0),
-                              k_pages.stride(1), v_pages.data_ptr(), v_pages.stride(0), v_pages.stride(1), table.data_ptr(), ld,
-                              table.shape[1], lens.data_ptr(), q_start.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), N, B,
-                              Hq, Hk, D, page, n, max_q, max_k, scale, int(causal), _p(ws), ws_bytes), "avsr_paged_attn")
+    ot, oh, _ = out.stride()
+    rc = lib.avsr_paged_attn(stream, dt, q.data_ptr(), qt, qh, k_pages.data_ptr(), kp, kh, v_pages.data_ptr(), vp, vh, table.data_ptr(), ld, W,
+                             lens.data_ptr(), q_start.data_ptr(), out.data_ptr(), ot, oh, N, B, Hq, Hk, D, page, n, max_q, max_k, scale,
+                             bool(causal), _p(ws), ws_bytes)
+    check(rc, "avsr_paged_attn")
     return out
 
 
@@ -1171,34 +1193,39 @@ def w4_quantize(weight, group=64):
 def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=None):
     """act(x @ w^T + bias) + residual for x [M, K] (fp32 or bf16) and a ``W4Weight``: [M, N] of ``out_dtype`` (x's type).
     ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself."""
-    lib = _lib.load()
-    N, K, group = w.N, w.K, w.group
-    T, C = -(-N // 16), -(-K // 128)
-    if (group not in W4_GROUPS or w.packed.dtype != torch.int32 or w.packed.numel() != T * C * 256 or w.scales.dtype != torch.bfloat16
-            or w.scales.numel() != T * 16 * (C * 128 // group) or not w.packed.is_contiguous() or not w.scales.is_contiguous()):
+    packed, scales, N, K, group = w
+    T, C = (N + 15) // 16, (K + 127) // 128
+    if (group not in W4_GROUPS or packed.dtype is not torch.int32 or packed.numel() != T * C * 256 or scales.dtype is not torch.bfloat16
+            or scales.numel() * group != T * C * 2048 or not packed.is_contiguous() or not scales.is_contiguous()):
         raise ValueError("not a W4Weight of its N, K and group (see w4_pack)")
-    if x.dim() != 2 or x.shape[1] != K or x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < K):
-        raise ValueError(f"x must be [M, {K}] with unit inner stride")
+    if x.dim() != 2 or x.shape[1] != K:
+        raise ValueError(f"x must be [M, {K}]")
     M = x.shape[0]
-    odt = out_dtype if out_dtype is not None else (out.dtype if out is not None else x.dtype)
+    ldx, one = x.stride()
+    odt = out_dtype or (x.dtype if out is None else out.dtype)
     if odt not in _DT:
         raise TypeError(f"unsupported dtype {odt}")
+    ldr = N
     for t, what in ((out, "out"), (residual, "residual")):
-        if t is not None and (t.dtype != odt or tuple(t.shape) != (M, N) or t.stride(1) != 1 or (M > 1 and t.stride(0) < N)):
-            raise ValueError(f"{what} must be a row-major [{M}, {N}] tensor of type {odt}")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (N,) or not bias.is_contiguous()):
-        raise ValueError("bias must be contiguous fp32 [N]")
-    if act not in (ACT_NONE, ACT_GELU, ACT_RELU):
+        if t is not None:
+            if t.dtype is not odt or t.shape != (M, N) or t.stride(1) != 1 or (M > 1 and t.stride(0) < N):
+                raise ValueError(f"{what} must be a row-major [{M}, {N}] tensor of type {odt}")
+            ldr = t.stride(0) if M > 1 else N
+    if one != 1 and K > 1 or (M > 1 and ldx < K):
+        raise ValueError("x needs unit inner stride")
+    if bias is not None and (bias.dtype is not torch.float32 or bias.shape != (N,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous fp32 [{N}]")
+    if act != ACT_NONE and act != ACT_GELU and act != ACT_RELU:
         raise ValueError("act must be ACT_NONE, ACT_GELU or ACT_RELU")
-    _same_gpu(x, w.packed, w.scales, bias, residual, out)
+    xdt = _dt(x)
+    stream = _gpu_stream(x, packed, scales, bias, residual, out)
     if out is None:
         out = torch.empty((M, N), dtype=odt, device=x.device)
     if M == 0:
         return out
-    row = lambda t: t.stride(0) if M > 1 else t.shape[1]
-    check(lib.avsr_w4_matmul(_stream(), _dt(x), _DT[odt], x.data_ptr(), row(x), w.packed.data_ptr(), w.scales.data_ptr(), group, _p(bias),
-                             act, _p(residual), 0 if residual is None else row(residual), out.data_ptr(), row(out), M, N, K),
-          "avsr_w4_matmul")
+    rc = _lib.load().avsr_w4_matmul(stream, xdt, _DT[odt], x.data_ptr(), ldx if M > 1 else K, packed.data_ptr(), scales.data_ptr(), group,
+                                    _p(bias), act, _p(residual), ldr, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K)
+    check(rc, "avsr_w4_matmul")
     return out
 
 

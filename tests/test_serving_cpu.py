@@ -100,7 +100,7 @@ def test_c_entries_refuse_before_they_launch():
     plan = lambda B=2, page=16, width=3, ld=3, n=4, tokens=8, ws=p, lens=p: lib.avsr_paged_plan(
         None, lens, p, p, ld, width, p, n, p, B, page, tokens, p, p, p, p, p, p, ws)
     assert plan(lens=None) == -1 and plan(B=0) == -1 and plan(ld=2) == -1 and plan(tokens=0) == -1 and plan(n=0) == -1
-    assert plan(B=5000, ws=None) == -1 and lib.avsr_paged_plan_workspace_bytes(5000, 8) > 0
+    assert plan(B=5000, ws=None) == -1 and lib.avsr_paged_plan_workspace_bytes(5000, 8, 4) > 0
     assert plan(page=17) == -2 and plan(page=8) == -2 and plan(n=1 << 27) == -2 and plan(width=1 << 27, ld=1 << 27) == -2
     write = lambda it=1, ot=1, k=p, ldk=128, D=64, page=16, slots=p, n=4: lib.avsr_paged_write(
         None, it, ot, k, ldk, 64, p, 128, 64, p, 2048, 1024, p, 2048, 1024, slots, 3, 2, D, page, n)
@@ -112,7 +112,7 @@ def test_c_entries_refuse_before_they_launch():
     assert attn(D=80) == -2 and attn(page=20) == -2 and attn(ldq=258) == -2 and attn(q=p + 8) == -2 and attn(N=1 << 29) == -2
     long = lambda ws, wb: lib.avsr_paged_attn(None, 1, p, 256, 64, p, 4096, 1024, p, 4096, 1024, p, 999, 999, p, p, p, 256, 64, 2, 2, 4, 2, 64,
                                               16, 9, 1, 15984, 1.0, 1, ws, wb)
-    need = lib.avsr_paged_attn_workspace_bytes(2, 2, 4, 2, 64, 1, 15984)
+    need = lib.avsr_paged_attn_workspace_bytes(1, 2, 2, 4, 2, 64, 1, 15984)
     assert need > 0 and long(None, 0) == -1 and long(p, need - 1) == -1
     w4 = lambda xt=1, ot=1, x=p, ldx=64, group=32, act=0, ldy=32, packed=p, K=64: lib.avsr_w4_matmul(
         None, xt, ot, x, ldx, packed, p, group, None, act, None, 0, p, ldy, 2, 32, K)

@@ -79,6 +79,18 @@ def test_plan_refuses_a_step_as_a_whole(dev, B, what, status):
         assert run_plan(dev, lens, new, table, ring, pool, page, cap, in_place) == want
 
 
+@pytest.mark.parametrize("n", [100, (1 << 20) + 5])
+def test_plan_sums_that_leave_32_bits(dev, n):
+    """Wide table rows (never touched) and requests of millions of pages: the status of exact sums, and nothing is written."""
+    B, page, width = 40, 16, 1 << 23
+    table = torch.zeros(B, width, dtype=torch.int32, device=dev)
+    for lens, new, status in (([0] * B, [1 << 27] * B, 1 | 4), ([1 << 27] * B, [-1] * B, 8), ([1 << 27] * B, [0] * B, 0), ([0] * B, [2 ** 31 - 1] * B, 2)):
+        held, pool = i32(lens, dev), i32([0, 90], dev)
+        plan = ops.paged_plan(held, i32(new, dev), table, torch.zeros(n, dtype=torch.int32, device=dev), pool, page, 64)
+        assert plan.status.item() == status
+        assert held.tolist() == lens and pool.tolist() == [0, 90] and plan.q_start.tolist() == [0] * (B + 1)
+
+
 def test_plan_takes_rows_of_a_wider_table(dev):
     wide = torch.full((4, 9), -5, dtype=torch.int32, device=dev)
     lens, ring, pool = i32([0, 3, 16, 0], dev), torch.arange(8, dtype=torch.int32, device=dev), i32([0, 6], dev)
