@@ -7,7 +7,6 @@
 // A page holds `page` tokens of one layer: element (p, h, t, d) of the keys lives at K + p*sp + h*sh + t*D + d, the
 // values in the same way (the [page, D] block of a page and head is contiguous, page and head strides are free).
 #include "common.h"
-#include <type_traits>
 
 #define LOG2E 1.4426950408889634f
 
@@ -812,11 +811,15 @@ template <int TR> __device__ __forceinline__ RowTile row_tile(const AttnArgs& a,
         Req r = {0, 0, 0};
         if (lane < a.B) r = request(a, lane);
         const int mine = r.nq * a.G > a.few_rows ? (r.nq * a.G + TR - 1) / TR : 0;
-        int before = 0;
+        int before = 0, total = 0;
         for (int j = 0; j < a.B; ++j) {
             const int len = __builtin_amdgcn_readlane(r.len, j), n = __builtin_amdgcn_readlane(mine, j);
             before += len > r.len || (len == r.len && j < lane) ? n : 0;
+            total += n;
         }
+        // the workgroups that start together on a CU: one of the longest, one of the shortest, one from between
+        const int round = max(1, 256 / (a.Hk * a.splits));
+        if (tile >= round && tile < total) tile = tile < 2 * round ? total - 1 - (tile - round) : tile - round;
         const unsigned long long who = __ballot(tile >= before && tile < before + mine);
         t.b = who ? __builtin_ctzll(who) : 0;
         start = who ? __builtin_amdgcn_readlane(before, t.b) : 1 << 30;      // no such tile
@@ -895,6 +898,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
+__device__ __forceinline__ float max16(const f32x16& s) {
+    float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]);
+    a = max3(a, s[6], s[7]); b = max3(b, s[8], s[9]);
+    a = max3(a, s[10], s[11]); b = max3(b, s[12], s[13]);
+    return max3(max3(a, s[14], s[15]), b, b);
+}
 template <int D> struct KvTile {
     static constexpr int CH = D / 8;                                  // 16-byte chunks of a key row
     static constexpr int PIECES = 16 * CH / 64;                       // DMA instructions of 16 keys
@@ -942,11 +951,8 @@ __device__ __forceinline__ u32x4 finite_part(u32x4 v, bool& odd) {
     return v;
 }
 
-#ifndef CHUNK_UNROLL
-#define CHUNK_UNROLL 2
-#endif
 #ifndef CHUNK_NBUF
-#define CHUNK_NBUF (D == 64 ? 3 : 2)
+#define CHUNK_NBUF 2
 #endif
 #ifndef CHUNK_OCC
 #define CHUNK_OCC (D == 64 ? 3 : 2)
@@ -966,9 +972,9 @@ __global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnAr
     const int wg_rows = min(128 * RT, rt.rows - rt.r0);
     const int base = a.causal ? r.len - r.nq : r.len - 1;
     const int kmax_wg = a.causal ? base + (rt.r0 + wg_rows - 1) / a.G : base;      // the last key of the workgroup's rows
+    const int kmin_wg = a.causal ? base + rt.r0 / a.G : base;                       // the last key that all of them see
     // this wave's rows; a wave without any helps to move the tiles
     const int r0 = rt.r0 + w * 32 * RT, n_rows = max(0, min(32 * RT, rt.rows - r0));
-    const int kmin = n_rows == 0 ? -1 : a.causal ? base + r0 / a.G : base;
     const int kmax = n_rows == 0 ? -1 : a.causal ? base + (r0 + n_rows - 1) / a.G : base;
     bf16x8 q[RT][D / 16];
     int limit[RT];
@@ -1025,6 +1031,7 @@ __global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnAr
         if (((kt * 64 + 48) >> a.shift) - first >= 64) {
             first = kt * 64 >> a.shift;
             entries = row[min(first + lane, a.width - 1)];
+            asm volatile("" : "+v"(entries));             // its wait belongs in here: outside it would drain the DMA every time
         }
         int p[4];
 #pragma unroll
@@ -1047,18 +1054,92 @@ __global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnAr
         for (int u = 0; u < NBUF - 1; ++u)
             if (t0 + u < t1) move(t0 + u, u, u);
     }
-    for (int kt = t0, buf = 0; kt < t1; ++kt, buf = buf == NBUF - 1 ? 0 : buf + 1) {
-        // this wave's part of the tile is in LDS (a younger tile may still be on its way) ...
+    int kt = t0, buf = 0;
+    // Tile kt is in LDS for every wave, and a younger one on its way into the buffer that is free; which of its runs have pages.
+    auto arrive = [&]() {
         if (NBUF == 3 && kt + 1 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * L::PIECES) : "memory");
-        else if (NBUF == 4 && kt + 2 < t1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(4 * L::PIECES) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                                          // ... and everyone's, and the buffer before it is free
+        __syncthreads();
         const unsigned have = pages & 15u;
         pages >>= 4;
         if (kt + NBUF - 1 < t1) move(kt + NBUF - 1, buf == 0 ? NBUF - 1 : buf - 1, NBUF - 2);
-        if (kt * 64 > kmax) continue;                             // none of this wave's rows sees the tile
-        auto half = [&](int st, auto whole_tile) {                // 32 of the tile's keys
-            constexpr bool whole = decltype(whole_tile)::value;
+        return have;
+    };
+        // the reference point of row tile n moves to the row's maximum so far (rare after the first tiles)
+        auto move_reference = [&](int n, float mx) {
+            const unsigned u = __builtin_bit_cast(unsigned, mx);
+            const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            const float top = fmaxf(m[n], fmaxf(__builtin_bit_cast(float, (unsigned)sw[0]), __builtin_bit_cast(float, (unsigned)sw[1])));
+            const float al = top > m[n] ? __builtin_amdgcn_exp2f((m[n] - top) * c) : 1.f;
+            m[n] = top;
+            thr[n] = top + lazy;
+            nm[n] = top == -INFINITY ? 0.f : -(top * c);
+            l[n] *= al;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[n][d][x] *= al;
+        };
+        // Scores to probabilities: rounded to bf16 for the product (half a step of 2^-8 relative each); the sum is of the unrounded ones.
+        auto exponentials = [&](int n, f32x16& s, bf16x8 (&p)[2]) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int x = 0; x < 16; x += 2) {
+                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], c, nm[n]));
+                s[x + 1] = __builtin_amdgcn_exp2f(fmaf(s[x + 1], c, nm[n]));
+                s0 += s[x];
+                s1 += s[x + 1];
+            }
+            l[n] += s0 + s1;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) { p[0][x] = (bf16_t)s[x]; p[1][x] = (bf16_t)s[8 + x]; }
+        };
+        // A tile that every row sees whole, 64 keys at once: one look at the maximum, and the matrix pipe has the other half's
+        // products to do while the vector unit makes the exponentials of one.
+        auto whole_tile = [&]() {
+            const char *K = (const char*)Ks[buf], *V = (const char*)Vs[buf];
+            f32x16 s[2][RT];
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int n = 0; n < RT; ++n)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) s[st][n][x] = 0.f;
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    const bf16x8 kf = L::kfrag(K + st * 64 * D, kr[ks]);
+#pragma unroll
+                    for (int n = 0; n < RT; ++n) s[st][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, q[n][ks], s[st][n], 0, 0, 0);
+                }
+            float mx[RT];
+            bool up = false;
+#pragma unroll
+            for (int n = 0; n < RT; ++n) {
+                mx[n] = fmaxf(max16(s[0][n]), max16(s[1][n]));
+                up |= mx[n] > thr[n];
+            }
+            if (__any(up)) {
+#pragma unroll
+                for (int n = 0; n < RT; ++n) move_reference(n, mx[n]);
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+                bf16x8 p[RT][2];
+#pragma unroll
+                for (int n = 0; n < RT; ++n) exponentials(n, s[st][n], p[n]);
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+                    for (int d = 0; d < D / 32; ++d) {
+                        const bf16x8 vf = L::vfrag(V + st * 64 * D, s2, vr[d]);
+#pragma unroll
+                        for (int n = 0; n < RT; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[n][s2], o[n][d], 0, 0, 0);
+                    }
+            }
+        };
+        auto half = [&](int st, unsigned have) {                  // 32 keys of a tile that some row sees in part
             const char *K = (const char*)Ks[buf] + st * 64 * D, *V = (const char*)Vs[buf] + st * 64 * D;
             const int k0 = kt * 64 + 32 * st;
             const bool ok0 = have >> (2 * st) & 1, ok1 = have >> (2 * st + 1) & 1;
@@ -1076,44 +1157,14 @@ __global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnAr
             bf16x8 p[RT][2];
 #pragma unroll
             for (int n = 0; n < RT; ++n) {
-                if constexpr (!whole) {
 #pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const int key = (x & 3) + 8 * (x >> 2) + 4 * hf;
-                        if (k0 + key > limit[n] || !(x < 8 ? ok0 : ok1)) s[n][x] = -INFINITY;
-                    }
+                for (int x = 0; x < 16; ++x) {
+                    const int key = (x & 3) + 8 * (x >> 2) + 4 * hf;
+                    if (k0 + key > limit[n] || !(x < 8 ? ok0 : ok1)) s[n][x] = -INFINITY;
                 }
-                float mx = max3(s[n][0], s[n][1], s[n][2]), my = max3(s[n][3], s[n][4], s[n][5]);
-                mx = max3(mx, s[n][6], s[n][7]); my = max3(my, s[n][8], s[n][9]);
-                mx = max3(mx, s[n][10], s[n][11]); my = max3(my, s[n][12], s[n][13]);
-                mx = max3(mx, s[n][14], s[n][15]);
-                mx = max3(mx, my, my);
-                if (__any(mx > thr[n])) {                         // rare after the first tiles
-                    const unsigned u = __builtin_bit_cast(unsigned, mx);
-                    const auto sw = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-                    const float top = fmaxf(m[n], fmaxf(__builtin_bit_cast(float, (unsigned)sw[0]), __builtin_bit_cast(float, (unsigned)sw[1])));
-                    const float al = top > m[n] ? __builtin_amdgcn_exp2f((m[n] - top) * c) : 1.f;
-                    m[n] = top;
-                    thr[n] = top + lazy;
-                    nm[n] = top == -INFINITY ? 0.f : -(top * c);
-                    l[n] *= al;
-#pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) o[n][d][x] *= al;
-                }
-                float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-                for (int x = 0; x < 16; x += 2) {
-                    s[n][x] = __builtin_amdgcn_exp2f(fmaf(s[n][x], c, nm[n]));
-                    s[n][x + 1] = __builtin_amdgcn_exp2f(fmaf(s[n][x + 1], c, nm[n]));
-                    s0 += s[n][x];
-                    s1 += s[n][x + 1];
-                }
-                l[n] += s0 + s1;
-                // rounding to bf16 for the product: half a step of 2^-8 relative per probability; the sum l is of the unrounded ones
-#pragma unroll
-                for (int x = 0; x < 8; ++x) { p[n][0][x] = (bf16_t)s[n][x]; p[n][1][x] = (bf16_t)s[n][8 + x]; }
+                const float mx = max16(s[n]);
+                if (__any(mx > thr[n])) move_reference(n, mx);
+                exponentials(n, s[n], p[n]);
             }
             // In a tile that some row sees in part, values behind every row's last key are cleared, and ones that are not
             // finite (0 * inf for a row that does not see them) are added to the rows that do.
@@ -1123,11 +1174,11 @@ __global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnAr
 #pragma unroll
                 for (int d = 0; d < D / 32; ++d) {
                     bf16x8 vf = L::vfrag(V, s2, vr[d]);
-                    if constexpr (!whole) vf = __builtin_bit_cast(bf16x8, finite_part(cut_keys(__builtin_bit_cast(u32x4, vf), k0 + 16 * s2, hf, (s2 ? ok1 : ok0) ? kmax : -1), odd));
+                    vf = __builtin_bit_cast(bf16x8, finite_part(cut_keys(__builtin_bit_cast(u32x4, vf), k0 + 16 * s2, hf, (s2 ? ok1 : ok0) ? kmax : -1), odd));
 #pragma unroll
                     for (int n = 0; n < RT; ++n) o[n][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, p[n][s2], o[n][d], 0, 0, 0);
                 }
-            if (!whole && __any(odd)) {
+            if (__any(odd)) {
 #pragma unroll 1
                 for (int key = 0; key < 32; ++key)
 #pragma unroll
@@ -1145,13 +1196,19 @@ __global__ __launch_bounds__(256, CHUNK_OCC) void paged_attn_chunk_kernel(AttnAr
                         }
             }
         };
-        if (kt * 64 + 63 <= kmin && have == 15u) {                // every row sees all of it
-#pragma unroll CHUNK_UNROLL
-            for (int st = 0; st < 2; ++st) half(st, std::true_type{});
-        } else {
+    // two loops: with one, the accumulators would be copied where its two branches meet, for every tile
+    unsigned have = 15u;
+    for (; kt < t1; ++kt, buf = buf == NBUF - 1 ? 0 : buf + 1) {
+        if (kt * 64 + 63 > kmin_wg) break;
+        have = arrive();
+        if (have != 15u) break;
+        whole_tile();
+    }
+    for (bool here = have != 15u; kt < t1; ++kt, buf = buf == NBUF - 1 ? 0 : buf + 1, here = false) {
+        if (!here) have = arrive();
+        if (kt * 64 > kmax) continue;                             // none of this wave's rows sees the tile
 #pragma unroll 1
-            for (int st = 0; st < 2; ++st) half(st, std::false_type{});
-        }
+        for (int st = 0; st < 2; ++st) half(st, have);
     }
 #pragma unroll
     for (int n = 0; n < RT; ++n) {
