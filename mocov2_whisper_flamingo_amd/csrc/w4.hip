@@ -17,41 +17,39 @@
 struct W4Args {
     const u32x4* w; const bf16_t* scales; const void* x; long ldx; const float* bias; const void* residual; long ldr; void* y; long ldy;
     int M, N, K, chunks, tiles, act, out_f32, vec_x, vec_y;
+    int kw, block;                 // staged kernel: ways that share the columns (a power of two), chunks of x in LDS at once
 };
 
+// Eight values of x as matrix operands: bf16 as it is, fp32 as the exact sum of three bf16 values (8 + 8 + 8 bits of
+// significand, each cut off, not rounded).
 template <typename TX> struct XFrag;
 template <> struct XFrag<bf16_t> {
     static constexpr int P = 1;
-    bf16x8 p[1];
-    __device__ __forceinline__ void load(const bf16_t* x, int n, bool vec) {          // n: how many of the eight exist
-        if (vec && n >= 8) { p[0] = *(const bf16x8*)x; return; }
+    bf16x8 v;
+    __device__ __forceinline__ void load(const bf16_t* x) { v = *(const bf16x8*)x; }
+    __device__ __forceinline__ void load(const bf16_t* x, int n) {                    // the first n of the eight, wherever they stand
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[0][j] = j < n ? x[j] : (bf16_t)0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? x[j] : (bf16_t)0.f;
     }
-    __device__ __forceinline__ bf16x8 piece(int) const { return p[0]; }
+    __device__ __forceinline__ bf16x8 piece(int) const { return v; }
 };
-// fp32 activations are the exact sum of three bf16 values (8 + 8 + 8 bits of significand, each cut off, not rounded)
 template <> struct XFrag<float> {
     static constexpr int P = 3;
-    float v[8];
-    __device__ __forceinline__ void load(const float* x, int n, bool vec) {
-        if (vec && n >= 8) {
-            const f32x4 a = *(const f32x4*)x, b = *(const f32x4*)(x + 4);
+    f32x4 a, b;
+    __device__ __forceinline__ void load(const float* x) { a = *(const f32x4*)x; b = *(const f32x4*)(x + 4); }
+    __device__ __forceinline__ void load(const float* x, int n) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
-            return;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < n ? x[j] : 0.f;
+        for (int j = 0; j < 4; ++j) { a[j] = j < n ? x[j] : 0.f; b[j] = 4 + j < n ? x[4 + j] : 0.f; }
     }
-    static __device__ __forceinline__ float cut(float a) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, a) & 0xFFFF0000u); }
+    // what three cuts leave of an infinity is NaN, like the sums it goes into
+    static __device__ __forceinline__ float cut(float f) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, f) & 0xFFFF0000u); }
     __device__ __forceinline__ bf16x8 piece(int i) const {
         u32x4 o;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float a = v[2 * j], b = v[2 * j + 1];
-            for (int q = 0; q < i; ++q) { a -= cut(a); b -= cut(b); }
-            o[j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, b), __builtin_bit_cast(unsigned, a), 0x07060302u);
+            float x = j < 2 ? a[2 * j] : b[2 * j - 4], y = j < 2 ? a[2 * j + 1] : b[2 * j - 3];
+            for (int q = 0; q < i; ++q) { x -= cut(x); y -= cut(y); }
+            o[j] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, y), __builtin_bit_cast(unsigned, x), 0x07060302u);
         }
         return __builtin_bit_cast(bf16x8, o);
     }
@@ -66,42 +64,32 @@ __device__ __forceinline__ bf16x8 w4_operand(unsigned w) {      // 16 + nibble, 
     return __builtin_bit_cast(bf16x8, o);
 }
 
-// NT tiles of 16 weight rows, MT tiles of 16 activation rows; GS: 32-column steps of a scale group (1, 2, 4).
-// The waves of a workgroup take the 128-column chunks in turn and are added up through LDS.
-#define W4_MAX_WAVES 8
-template <typename TX, int GS, int MT, int NT>
-__global__ __launch_bounds__(64 * W4_MAX_WAVES) void w4_matmul_kernel(W4Args a) {
-    extern __shared__ f32x4 s_part[];                            // [waves][NT * MT][64]
-    constexpr int NG = 4 / GS;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int i = lane & 15, g = lane >> 4;
-    const int t0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT;
+// A wave's share: NT tiles of 16 weight rows times MT tiles of 16 rows of x; GS: 32-column steps of a scale group (1, 2, 4).
+template <int GS, int MT, int NT> struct W4Wave {
+    static constexpr int NG = 4 / GS;
+    struct W { u32x4 w[NT]; bf16x4 sc[NT][NG]; };                // 128 columns of the weights
+    const u32x4* wp[NT];
+    const bf16_t* sp[NT];
     f32x4 tot[NT][MT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) tot[n][m] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    struct Stage { u32x4 w[NT]; bf16x4 sc[NT][NG]; XFrag<TX> x[MT][4]; };
-    auto load = [&](Stage& st, int c) {
+    __device__ __forceinline__ W4Wave(const W4Args& a, int t0, int lane) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const long t = min(t0 + n, a.tiles - 1);
-            st.w[n] = a.w[(t * a.chunks + c) * 64 + lane];
+            const long t = min(t0 + n, a.tiles - 1);             // a tile behind the last is computed like it and not stored
+            wp[n] = a.w + t * a.chunks * 64 + lane;
+            sp[n] = a.scales + t * a.chunks * NG * 16 + 4 * (lane >> 4);
 #pragma unroll
-            for (int q = 0; q < NG; ++q) st.sc[n][q] = *(const bf16x4*)(a.scales + ((t * a.chunks + c) * NG + q) * 16 + 4 * g);
+            for (int m = 0; m < MT; ++m) tot[n][m] = (f32x4){0.f, 0.f, 0.f, 0.f};
         }
+    }
+    __device__ __forceinline__ void load(W& st, int c) const {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            const int row = m0 + 16 * m + i;
+        for (int n = 0; n < NT; ++n) {
+            st.w[n] = wp[n][c * 64];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int k = c * 128 + 32 * s + 8 * g;
-                const int n = row < a.M ? a.K - k : 0;
-                st.x[m][s].load((const TX*)a.x + (n > 0 ? row * a.ldx + k : 0), n, a.vec_x);
-            }
+            for (int q = 0; q < NG; ++q) st.sc[n][q] = *(const bf16x4*)(sp[n] + (c * NG + q) * 16);
         }
-    };
-    auto compute = [&](const Stage& st) {
+    }
+    template <int P, typename X> __device__ __forceinline__ void add(const W& st, X x) {      // x(m, s, p): operand of step s, piece p
         bf16x8 minus;
 #pragma unroll
         for (int j = 0; j < 8; ++j) minus[j] = (bf16_t)-24.f;
@@ -118,50 +106,57 @@ __global__ __launch_bounds__(64 * W4_MAX_WAVES) void w4_matmul_kernel(W4Args a) 
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                f32x4 base = (f32x4){0.f, 0.f, 0.f, 0.f};
-                bf16x8 xs[GS][XFrag<TX>::P];
+                f32x4 base = (f32x4){0.f, 0.f, 0.f, 0.f}, acc[NT];
+                bf16x8 xs[GS][P];
 #pragma unroll
                 for (int s = 0; s < GS; ++s)
 #pragma unroll
-                    for (int p = 0; p < XFrag<TX>::P; ++p) {
-                        xs[s][p] = st.x[m][q * GS + s].piece(p);
+                    for (int p = 0; p < P; ++p) {
+                        xs[s][p] = x(m, q * GS + s, p);
                         base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus, xs[s][p], base, 0, 0, 0);
                     }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    f32x4 acc = base;
+                for (int n = 0; n < NT; ++n) acc[n] = base;
 #pragma unroll
-                    for (int s = 0; s < GS; ++s)
+                for (int s = 0; s < GS; ++s)
 #pragma unroll
-                        for (int p = 0; p < XFrag<TX>::P; ++p) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wo[n][s], xs[s][p], acc, 0, 0, 0);
+                    for (int p = 0; p < P; ++p)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) tot[n][m][r] = fmaf(sc[n][r], acc[r], tot[n][m][r]);
-                }
+                        for (int n = 0; n < NT; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wo[n][s], xs[s][p], acc[n], 0, 0, 0);
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) tot[n][m][r] = fmaf(sc[n][r], acc[n][r], tot[n][m][r]);
             }
         }
-    };
-    Stage st[2];
-    if (wave < a.chunks) load(st[0], wave);
-    for (int c = wave; c < a.chunks; c += 2 * waves) {
-        if (c + waves < a.chunks) load(st[1], c + waves);
-        compute(st[0]);
-        if (c + waves < a.chunks) {
-            if (c + 2 * waves < a.chunks) load(st[0], c + 2 * waves);
-            compute(st[1]);
-        }
     }
+    // The kw waves that share these tiles add up through LDS (room for all waves' sums); part p finishes every kw-th tile.
+    __device__ __forceinline__ void finish(const W4Args& a, f32x4* sum, int t0, int m0, int wave, int part, int kw, int lane) {
+        if (kw > 1) {
+            __syncthreads();
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) s_part[(wave * (NT * MT) + n * MT + m) * 64 + lane] = tot[n][m];
-    __syncthreads();
-    for (int j = threadIdx.x; j < NT * MT * 64; j += blockDim.x) {
-        f32x4 v = s_part[j];
-        for (int u = 1; u < waves; ++u) v += s_part[u * (NT * MT * 64) + j];
-        const int nm = j >> 6, l = j & 63;
-        const int row = m0 + 16 * (nm % MT) + (l & 15), n0 = (t0 + nm / MT) * 16 + 4 * (l >> 4);
-        if (row >= a.M || n0 >= a.N) continue;
+                for (int m = 0; m < MT; ++m) sum[(wave * NT * MT + n * MT + m) * 64 + lane] = tot[n][m];
+            __syncthreads();
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                if ((n * MT + m) % kw != part) continue;
+                f32x4 v = tot[n][m];
+                if (kw > 1) {
+                    const f32x4* p = sum + ((wave - part) * NT * MT + n * MT + m) * 64 + lane;
+                    v = p[0];
+                    for (int u = 1; u < kw; ++u) v += p[u * NT * MT * 64];
+                }
+                store(a, v, m0 + 16 * m + (lane & 15), (t0 + n) * 16 + 4 * (lane >> 4));
+            }
+    }
+    static __device__ __forceinline__ void store(const W4Args& a, f32x4 v, int row, int n0) {
         const int cnt = min(4, a.N - n0);
+        if (row >= a.M || cnt <= 0) return;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if (r >= cnt) break;
@@ -187,18 +182,139 @@ __global__ __launch_bounds__(64 * W4_MAX_WAVES) void w4_matmul_kernel(W4Args a) 
                 for (int r = 0; r < cnt; ++r) y[r] = (bf16_t)v[r];
         }
     }
+};
+
+// ---- x straight from L2: nothing to wait for before the first product.  The waves of a workgroup take the 128-column
+// chunks in turn.  A chunk's weights and scales (AHEAD: its x too) are loaded while the one before is multiplied.  Rows of x
+// behind the last are read as the last one: their columns of the product are never stored.
+#define W4_WAVES 8
+template <typename TX, int GS, int MT, int NT, bool AHEAD>
+__global__ __launch_bounds__(64 * W4_WAVES) void w4_direct_kernel(W4Args a) {
+    extern __shared__ f32x4 sums[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int t0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, g = lane >> 4;
+    W4Wave<GS, MT, NT> ww(a, t0, lane);
+    const TX* xp[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) xp[m] = (const TX*)a.x + (long)min(m0 + 16 * m + (lane & 15), a.M - 1) * a.ldx + 8 * g;
+    struct X { XFrag<TX> x[MT][4]; };
+    const int whole = a.vec_x ? a.K >> 7 : 0;                     // chunks whose x can be read in 16-byte pieces
+    auto load_x = [&](X& st, int c) {
+        if (c < whole) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) st.x[m][s].load(xp[m] + c * 128 + 32 * s);
+        } else {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int s = 0; s < 4; ++s) st.x[m][s].load(xp[m] + c * 128 + 32 * s, a.K - (c * 128 + 32 * s + 8 * g));
+        }
+    };
+    typename W4Wave<GS, MT, NT>::W sw[2];
+    X sx[AHEAD ? 2 : 1];
+    auto add = [&](int u) {
+        const X& x = sx[AHEAD ? u : 0];
+        ww.template add<XFrag<TX>::P>(sw[u], [&](int m, int s, int p) { return x.x[m][s].piece(p); });
+    };
+    // loads come back in order: x of a chunk is asked for before weights that are further ahead
+    if (AHEAD && wave < a.chunks) load_x(sx[0], wave);
+    if (wave < a.chunks) ww.load(sw[0], wave);
+    for (int c0 = wave; c0 < a.chunks; c0 += 2 * waves) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int c = c0 + u * waves;
+            if (c >= a.chunks) break;
+            if (!AHEAD) load_x(sx[0], c);
+            if (c + waves < a.chunks) {
+                if (AHEAD) load_x(sx[AHEAD ? u ^ 1 : 0], c + waves);
+                ww.load(sw[u ^ 1], c + waves);
+            }
+            add(u);
+        }
+    }
+    ww.finish(a, sums, t0, m0, wave, wave, waves, lane);
 }
 
+// ---- x through LDS, for wide layers: read by every wave for its own columns it takes up the vector memory path longer than
+// the weights do (16 rows: 4 KiB against 1 KiB a tile), here eight waves share it, and fp32 is taken apart once.  The waves
+// are kw ways of the chunks times 8 / kw groups of weight tiles.  x is staged in blocks of chunks, as many as fit, a row 16
+// bytes longer than its values so that the 16 rows a fragment reads lie in different banks.
+template <typename TX, int GS, int MT, int NT>
+__global__ __launch_bounds__(64 * W4_WAVES, XFrag<TX>::P == 1 || MT < 4 ? 4 : 2) void w4_staged_kernel(W4Args a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int P = XFrag<TX>::P;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int part = wave & (a.kw - 1), t0 = (blockIdx.x * (W4_WAVES / a.kw) + wave / a.kw) * NT, m0 = blockIdx.y * 16 * MT;
+    const int rows = min(16 * MT, a.M - m0), stride = a.block * 256 + 16;
+    W4Wave<GS, MT, NT> ww(a, t0, lane);
+    const char* xl[MT];                                          // rows behind the last are read as the last one
+#pragma unroll
+    for (int m = 0; m < MT; ++m) xl[m] = lds + min(16 * m + (lane & 15), rows - 1) * stride + 16 * (lane >> 4);
+    typename W4Wave<GS, MT, NT>::W sw[2];
+    for (int b0 = 0; b0 < a.chunks; b0 += a.block) {
+        const int b1 = min(a.chunks, b0 + a.block), first = b0 + part;
+        if (first < b1) ww.load(sw[0], first);
+        if (b0) __syncthreads();                                 // the block before has been read
+        const int pieces = (b1 - b0) * 16;                       // of eight values, of a row
+        for (int j = threadIdx.x; j < rows * pieces; j += 64 * W4_WAVES) {
+            const int row = j / pieces, pc = j - row * pieces, k = b0 * 128 + pc * 8;
+            const TX* x = (const TX*)a.x + (long)(m0 + row) * a.ldx + (k < a.K ? k : 0);
+            XFrag<TX> f;
+            if (a.vec_x && k + 8 <= a.K) f.load(x);
+            else f.load(x, a.K - k);
+#pragma unroll
+            for (int p = 0; p < P; ++p) *(bf16x8*)(lds + (p * rows + row) * stride + pc * 16) = f.piece(p);
+        }
+        __syncthreads();
+        for (int c0 = first; c0 < b1; c0 += 2 * a.kw) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int c = c0 + u * a.kw;
+                if (c >= b1) break;
+                if (c + a.kw < b1) ww.load(sw[u ^ 1], c + a.kw);
+                const int at = (c - b0) * 256;
+                ww.template add<P>(sw[u], [&](int m, int s, int p) { return *(const bf16x8*)(xl[m] + p * rows * stride + at + s * 64); });
+            }
+        }
+    }
+    ww.finish(a, (f32x4*)lds, t0, m0, wave, part, a.kw, lane);
+}
+
+#define W4_FILL 4096            // waves that the chip is given: 16 per CU
+#define W4_WIDE 1024            // tiles of weight rows from which a wave takes two (enough waves all the same)
+#define W4_X_BYTES 65536        // x in LDS: two workgroups share a CU
 template <typename TX, int GS>
-static int launch_w4(hipStream_t s, const W4Args& a) {
+static int launch_w4(hipStream_t s, W4Args a) {
+    constexpr int P = XFrag<TX>::P;
+    const bool wide = a.tiles >= W4_WIDE;
     const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    const int nt = a.tiles >= 1024 ? 2 : 1;
-    const int waves = a.chunks >= 8 ? 8 : 4;
-    const dim3 grid((a.tiles + nt - 1) / nt, (a.M + 16 * mt - 1) / (16 * mt)), block(64 * waves);
-    const int lds = waves * nt * mt * 64 * 16;
-#define L(MT, NT) hipLaunchKernelGGL((w4_matmul_kernel<TX, GS, MT, NT>), grid, block, lds, s, a)
-    if (nt == 1) { if (mt == 1) L(1, 1); else if (mt == 2) L(2, 1); else L(4, 1); }
-    else { if (mt == 1) L(1, 2); else if (mt == 2) L(2, 2); else L(4, 2); }
+    if (wide && a.M >= 4) {
+        const int nt = mt == 1 ? 2 : 1, groups = (a.tiles + nt - 1) / nt, rows = a.M < 16 * mt ? a.M : 16 * mt;
+        const int most = (W4_X_BYTES / (rows * P) - 16) / 256, blocks = (a.chunks + most - 1) / most;
+        a.block = (a.chunks + blocks - 1) / blocks;              // blocks of one size
+        a.kw = 1;
+        while (a.kw < W4_WAVES && groups * a.kw * 2 <= W4_FILL && a.kw < a.block) a.kw *= 2;
+        const int xb = rows * P * (a.block * 256 + 16), sb = a.kw > 1 ? W4_WAVES * nt * mt * 1024 : 0, lds = xb > sb ? xb : sb;
+        const int tw = W4_WAVES / a.kw;
+        const dim3 grid((groups + tw - 1) / tw, (a.M + 16 * mt - 1) / (16 * mt)), block(64 * W4_WAVES);
+#define L(MT, NT) hipLaunchKernelGGL((w4_staged_kernel<TX, GS, MT, NT>), grid, block, lds, s, a)
+        if (mt == 1) L(1, 2); else if (mt == 2) L(2, 1); else L(4, 1);
+#undef L
+        return avsr_launch_status();
+    }
+    const int nt = wide ? 2 : 1, groups = (a.tiles + nt - 1) / nt, mt_d = P == 3 && mt == 4 ? 2 : mt;      // fp32: three times the registers
+    int waves = W4_FILL / groups;                                // no more than there are chunks
+    waves = waves < 1 ? 1 : waves > W4_WAVES ? W4_WAVES : waves;
+    waves = waves < a.chunks ? waves : a.chunks;
+    const dim3 grid(groups, (a.M + 16 * mt_d - 1) / (16 * mt_d)), block(64 * waves);
+    const int lds = waves > 1 ? waves * nt * mt_d * 1024 : 0;
+#define L(MT, NT) hipLaunchKernelGGL((w4_direct_kernel<TX, GS, MT, NT, (P * MT * NT <= 3)>), grid, block, lds, s, a)
+    if (nt == 2) L(1, 2);
+    else if (mt_d == 1) L(1, 1);
+    else if (mt_d == 2) L(2, 1);
+    else if constexpr (P == 1) L(4, 1);
 #undef L
     return avsr_launch_status();
 }
