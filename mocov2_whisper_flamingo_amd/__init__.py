@@ -9,8 +9,9 @@ from .transforms import VideoTransform
 from .gate_cross_attention import GatedCrossAttentionBlock, GatedCrossModalFusion, LayerNorm
 from .moco_visual_frontend import MoCoVisualFrontend
 from .utils import Decoder, PositionalEncoding
+from .paged_cache import PagedKVCache
 from .whisper_encoder import WhisperConfig, WhisperEncoder, WhisperModel
 from .whisper_decoder import WhisperDecoder
 
 __all__ = ["AVNet", "GatedCrossAttentionBlock", "GatedCrossModalFusion", "LayerNorm", "LogMelFrontend", "MoCoVisualFrontend",
-           "Decoder", "PositionalEncoding", "VideoTransform", "WhisperConfig", "WhisperDecoder", "WhisperEncoder", "WhisperModel", "ops"]
+           "Decoder", "PagedKVCache", "PositionalEncoding", "VideoTransform", "WhisperConfig", "WhisperDecoder", "WhisperEncoder", "WhisperModel", "ops"]

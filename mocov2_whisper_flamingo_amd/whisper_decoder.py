@@ -12,12 +12,33 @@ self-attention keys / values of earlier tokens kept in a cache (what HF's
 kernel taking the new tokens as the LAST queries of the cached sequence.
 ``cross_kv`` exposes the per-layer encoder projections so they are computed
 once per encoder output.
+
+``new_paged_cache`` + ``paged_admit`` + ``paged_step`` + ``paged_end`` serve requests
+of different lengths that come and go: a step takes each request's new tokens (a
+prompt, one token, none) as rows of one ragged batch over a cache in pages;
+``greedy_ragged`` decodes a list of prompts that way.  ``quantize`` keeps the
+layers' weights in 4 bits.
 """
 import torch
 import torch.nn as nn
 
 from . import ops
+from .paged_cache import PagedKVCache
 from .whisper_encoder import _Attention
+
+
+def _linear(x, w, **kw):
+    """x @ w^T with the epilogue of ``ops.gemm_nt``, for a weight matrix or its 4-bit form."""
+    return ops.w4_matmul(x, w, **kw) if isinstance(w, ops.W4Weight) else ops.gemm_nt(x, w, **kw)
+
+
+class PagedDecoderCache:
+    """What a server keeps for its requests: ``tokens`` (self-attention), ``frames`` (cross-attention, or None), and ``bad``, an int32
+    GPU flag that a token id or position outside the embedding tables sets."""
+
+    def __init__(self, tokens, frames, dtype, device):
+        self.tokens, self.frames, self.dtype = tokens, frames, dtype
+        self.bad = torch.zeros(1, dtype=torch.int32, device=device)
 
 
 class _DecoderLayer(nn.Module):
@@ -43,10 +64,11 @@ class WhisperDecoder(nn.Module):
         self.layer_norm = nn.LayerNorm(d)
         self._packed = None
         self._proj = None
+        self._w4 = None            # (group, with the vocabulary) of quantize()
 
     # ---- weight packing -------------------------------------------------
     def _versions(self, dtype):
-        return (dtype, sum(p._version for p in self.parameters()), next(self.parameters()).data_ptr())
+        return (dtype, self._w4, sum(p._version for p in self.parameters()), next(self.parameters()).data_ptr())
 
     def _pack(self, dtype):
         """Per weight version: q/k/v of the self-attention fused into one [3D, D] matrix, k/v of the
@@ -81,6 +103,14 @@ class WhisperDecoder(nn.Module):
                 "wfc1": cd(L.fc1.weight), "bfc1": f32(L.fc1.bias),
                 "wfc2": cd(L.fc2.weight), "bfc2": f32(L.fc2.bias),
             })
+            if self._w4 is not None:
+                lw = pk["layers"][-1]
+                lw["wqkv"] = torch.cat([a.q_proj.weight.detach() * s, a.k_proj.weight.detach(), a.v_proj.weight.detach()], 0)
+                lw["wq_x"] = x.q_proj.weight.detach() * s
+                lw["wo"], lw["wo_x"] = a.out_proj.weight, x.out_proj.weight
+                lw["wfc1"], lw["wfc2"] = L.fc1.weight, L.fc2.weight
+                for name in ("wqkv", "wo", "wq_x", "wo_x", "wfc1", "wfc2"):
+                    lw[name] = ops.w4_quantize(lw[name], self._w4[0])
         self._packed = (key, pk)
         return pk
 
@@ -116,19 +146,19 @@ class WhisperDecoder(nn.Module):
             cross_kv = self.cross_kv(encoder_hidden_states, dtype)
         for i, lw in enumerate(pk["layers"]):
             h = ops.layernorm_fwd(xs, *lw["ln1"], out_dtype=dtype)
-            qkv = ops.gemm_nt(h, lw["wqkv"], bias=lw["bqkv"]).view(B, T, 3 * D)
+            qkv = _linear(h, lw["wqkv"], bias=lw["bqkv"]).view(B, T, 3 * D)
             o = ops.attn_fwd(qkv[:, :, :D], qkv[:, :, D:2 * D], qkv[:, :, 2 * D:], H, key_mask=km, scale=1.0,
                              use_mfma=use_mfma, causal=True)
-            ops.gemm_nt(o.view(B * T, D), lw["wo"], bias=lw["bo"], residual=xs, out=xs)
+            _linear(o.view(B * T, D), lw["wo"], bias=lw["bo"], residual=xs, out=xs)
             if cross_kv is not None:
                 kv = cross_kv[i]
                 h = ops.layernorm_fwd(xs, *lw["lnx"], out_dtype=dtype)
-                q = ops.gemm_nt(h, lw["wq_x"], bias=lw["bq_x"]).view(B, T, D)
+                q = _linear(h, lw["wq_x"], bias=lw["bq_x"]).view(B, T, D)
                 o = ops.attn_fwd(q, kv[:, :, :D], kv[:, :, D:], H, scale=1.0, use_mfma=use_mfma)
-                ops.gemm_nt(o.view(B * T, D), lw["wo_x"], bias=lw["bo_x"], residual=xs, out=xs)
+                _linear(o.view(B * T, D), lw["wo_x"], bias=lw["bo_x"], residual=xs, out=xs)
             h = ops.layernorm_fwd(xs, *lw["ln2"], out_dtype=dtype)
-            f = ops.gemm_nt(h, lw["wfc1"], bias=lw["bfc1"], act=ops.ACT_GELU)
-            ops.gemm_nt(f, lw["wfc2"], bias=lw["bfc2"], residual=xs, out=xs)
+            f = _linear(h, lw["wfc1"], bias=lw["bfc1"], act=ops.ACT_GELU)
+            _linear(f, lw["wfc2"], bias=lw["bfc2"], residual=xs, out=xs)
         out = ops.layernorm_fwd(xs, *pk["lnf"], out_dtype=dtype)
         return (out.view(B, T, D),)
 
@@ -162,7 +192,7 @@ class WhisperDecoder(nn.Module):
         xs = ops.embed_tokens(input_ids, pk["tok"], pk["pos"], past=past)
         for i, lw in enumerate(pk["layers"]):
             h = ops.layernorm_fwd(xs, *lw["ln1"], out_dtype=dtype)
-            qkv = ops.gemm_nt(h, lw["wqkv"], bias=lw["bqkv"]).view(B, T, 3 * D)
+            qkv = _linear(h, lw["wqkv"], bias=lw["bqkv"]).view(B, T, 3 * D)
             kv = cache["kv"][i]
             for b in range(B):                                  # this step's keys | values behind the cached ones
                 ops.cast_rows(qkv[b, :, D:], kv[b, past:past + T])
@@ -170,16 +200,16 @@ class WhisperDecoder(nn.Module):
             if B > 1 and past + T < kv.shape[1]:                # the kernel's batch stride is Tk rows: pack the filled part
                 seen = seen.contiguous()
             o = ops.attn_fwd(qkv[:, :, :D], seen[:, :, :D], seen[:, :, D:], H, scale=1.0, use_mfma=use_mfma, causal=True)
-            ops.gemm_nt(o.view(B * T, D), lw["wo"], bias=lw["bo"], residual=xs, out=xs)
+            _linear(o.view(B * T, D), lw["wo"], bias=lw["bo"], residual=xs, out=xs)
             if cache["cross"] is not None:
                 ckv = cache["cross"][i]
                 h = ops.layernorm_fwd(xs, *lw["lnx"], out_dtype=dtype)
-                q = ops.gemm_nt(h, lw["wq_x"], bias=lw["bq_x"]).view(B, T, D)
+                q = _linear(h, lw["wq_x"], bias=lw["bq_x"]).view(B, T, D)
                 o = ops.attn_fwd(q, ckv[:, :, :D], ckv[:, :, D:], H, scale=1.0, use_mfma=use_mfma)
-                ops.gemm_nt(o.view(B * T, D), lw["wo_x"], bias=lw["bo_x"], residual=xs, out=xs)
+                _linear(o.view(B * T, D), lw["wo_x"], bias=lw["bo_x"], residual=xs, out=xs)
             h = ops.layernorm_fwd(xs, *lw["ln2"], out_dtype=dtype)
-            f = ops.gemm_nt(h, lw["wfc1"], bias=lw["bfc1"], act=ops.ACT_GELU)
-            ops.gemm_nt(f, lw["wfc2"], bias=lw["bfc2"], residual=xs, out=xs)
+            f = _linear(h, lw["wfc1"], bias=lw["bfc1"], act=ops.ACT_GELU)
+            _linear(f, lw["wfc2"], bias=lw["bfc2"], residual=xs, out=xs)
         cache["len"] = past + T
         return ops.layernorm_fwd(xs, *pk["lnf"], out_dtype=dtype).view(B, T, D)
 
@@ -209,8 +239,150 @@ class WhisperDecoder(nn.Module):
     def project_tokens(self, hidden, out_dtype=torch.float32):
         """Vocabulary logits with the tied output projection of HF ``WhisperForConditionalGeneration``
         (``proj_out.weight`` is ``embed_tokens.weight``, no bias): [B, T, D] -> [B, T, vocab]."""
-        key = (hidden.dtype, self.embed_tokens.weight._version, self.embed_tokens.weight.data_ptr())
+        w4 = self._w4 is not None and self._w4[1]
+        key = (hidden.dtype, w4 and self._w4, self.embed_tokens.weight._version, self.embed_tokens.weight.data_ptr())
         if self._proj is None or self._proj[0] != key:
-            self._proj = (key, self.embed_tokens.weight.detach().to(hidden.dtype).contiguous())
+            w = self.embed_tokens.weight.detach()
+            self._proj = (key, ops.w4_quantize(w, self._w4[0]) if w4 else w.to(hidden.dtype).contiguous())
         B, T, D = hidden.shape
-        return ops.gemm_nt(hidden.reshape(B * T, D), self._proj[1], out_dtype=out_dtype).view(B, T, -1)
+        return _linear(hidden.reshape(B * T, D), self._proj[1], out_dtype=out_dtype).view(B, T, -1)
+
+    # ---- 4-bit weights ------------------------------------------------------
+    def quantize(self, group=64, head=False):
+        """Keeps the layers' projections and MLPs (and with ``head`` the tied vocabulary projection) as 4-bit weights with a scale per
+        ``group`` columns (``ops.w4_quantize``: nearest), for every call from here on; ``group=None`` goes back to full weights.  The
+        parameters themselves, the encoder's key / value projections and the embeddings stay as they are."""
+        if group is not None and group not in ops.W4_GROUPS:
+            raise ValueError(f"group must be one of {ops.W4_GROUPS} or None")
+        self._w4 = None if group is None else (group, bool(head))
+        self._packed = self._proj = None
+        return self
+
+    # ---- requests of different lengths ---------------------------------------
+    def new_paged_cache(self, requests, *, pages=None, page_size=64, max_tokens=None, frames=None, frame_pages=None, dtype=torch.bfloat16,
+                        device=None):
+        """An empty cache for ``requests`` requests of up to ``max_tokens`` tokens (default and most: max_target_positions) over ``pages``
+        pages (default: enough for all of them).  ``frames``: most encoder frames of a request, over ``frame_pages`` pages; None: no
+        cross-attention."""
+        cfg = self.cfg
+        n = cfg.max_target_positions if max_tokens is None else int(max_tokens)
+        if n > cfg.max_target_positions or n < 1 or n % page_size:
+            raise ValueError(f"max_tokens must be a multiple of the page size, up to max_target_positions={cfg.max_target_positions}")
+        device = device or self.embed_tokens.weight.device
+        H, D = cfg.decoder_attention_heads, cfg.d_model // cfg.decoder_attention_heads
+        make = lambda most, count: PagedKVCache(len(self.layers), requests, H, D, max_tokens=most, page_size=page_size, dtype=dtype, device=device,
+                                                pages=requests * -(-most // page_size) if count is None else count)
+        return PagedDecoderCache(make(n, pages), None if frames is None else make(int(frames), frame_pages), dtype, device)
+
+    @torch.no_grad()
+    def paged_admit(self, cache, requests, encoder_hidden_states):
+        """Encoder output [n, Te, D] of the n given requests (ascending, none of which holds frames) into the cache's frames.  Raises if
+        the pages do not suffice, with nothing changed."""
+        if cache.frames is None:
+            raise ValueError("the cache was made without frames")
+        requests = [int(r) for r in requests]
+        n, Te, D = encoder_hidden_states.shape
+        if len(requests) != n or n == 0 or any(b <= a for a, b in zip(requests, requests[1:])) or requests[0] < 0 or requests[-1] >= cache.frames.requests:
+            raise ValueError("paged_admit expects one ascending request index per encoder output")
+        if bool((cache.frames.lens[requests] != 0).any()):
+            raise ValueError("a request that holds frames has to end first (paged_end)")
+        new = [0] * cache.frames.requests
+        for r in requests:
+            new[r] = Te
+        plan = cache.frames.plan(torch.tensor(new, dtype=torch.int32, device=cache.bad.device), n * Te)
+        cache.frames.check(plan)
+        H = self.cfg.decoder_attention_heads
+        for i, kv in enumerate(self.cross_kv(encoder_hidden_states, cache.dtype)):
+            kv = kv.view(n * Te, 2 * D)
+            cache.frames.write(i, kv[:, :D].unflatten(1, (H, -1)), kv[:, D:].unflatten(1, (H, -1)), plan)
+
+    @torch.no_grad()
+    def paged_step(self, cache, input_ids, new, max_new=None):
+        """One step of a server.  ``new``: tokens each request adds (0: it waits, -1: it ends and gives its tokens' pages back; its frames
+        go with :meth:`paged_end`); ``input_ids`` int64 [N]: these tokens, request after request.  Returns their hidden states [N, D],
+        the values :meth:`forward` gives for these positions of each request's sequence, and the step's plan.
+
+        ``new`` as a list is checked: the call waits for the GPU, and raises, with nothing changed, on ids outside the vocabulary and on
+        a step that does not fit.  As an int32 GPU tensor it is taken as it is, and the call can be recorded in a HIP graph (``max_new``:
+        at most so many new tokens of one request; default N): ``plan.status`` and ``cache.bad`` say whether it went well; rows behind
+        the last token hold nothing."""
+        cfg, dtype, tok = self.cfg, cache.dtype, cache.tokens
+        if input_ids.dim() != 1 or input_ids.dtype != torch.int64:
+            raise ValueError("input_ids must be int64 [tokens]")
+        N = input_ids.shape[0]
+        checked = not torch.is_tensor(new)
+        if checked:
+            new = [int(n) for n in new]
+            if len(new) != tok.requests or sum(max(n, 0) for n in new) != N:
+                raise ValueError(f"new must give each of the {tok.requests} requests its share of the {N} tokens")
+            if N and bool(((input_ids < 0) | (input_ids >= cfg.vocab_size)).any()):
+                raise IndexError("token id out of range for the embedding table")
+            max_new = max(new)
+            new = torch.tensor(new, dtype=torch.int32, device=cache.bad.device)
+        pk = self._pack(dtype)
+        plan = tok.plan(new, max(N, 1))
+        if checked:
+            tok.check(plan)
+        H, D = cfg.decoder_attention_heads, cfg.d_model
+        if N == 0:
+            return torch.empty((0, D), dtype=dtype, device=input_ids.device), plan
+        heads = lambda t: t.unflatten(1, (H, -1))
+        xs = ops.embed_tokens_at(input_ids, pk["tok"], pk["pos"], plan.positions, bad=cache.bad)
+        for i, lw in enumerate(pk["layers"]):
+            h = ops.layernorm_fwd(xs, *lw["ln1"], out_dtype=dtype)
+            qkv = _linear(h, lw["wqkv"], bias=lw["bqkv"])
+            tok.write(i, heads(qkv[:, D:2 * D]), heads(qkv[:, 2 * D:]), plan)
+            o = tok.attend(i, heads(qkv[:, :D]), plan.q_start, max_q=max_new)
+            _linear(o.view(N, D), lw["wo"], bias=lw["bo"], residual=xs, out=xs)
+            if cache.frames is not None:
+                h = ops.layernorm_fwd(xs, *lw["lnx"], out_dtype=dtype)
+                q = _linear(h, lw["wq_x"], bias=lw["bq_x"])
+                o = cache.frames.attend(i, heads(q), plan.q_start, max_q=max_new, causal=False)
+                _linear(o.view(N, D), lw["wo_x"], bias=lw["bo_x"], residual=xs, out=xs)
+            h = ops.layernorm_fwd(xs, *lw["ln2"], out_dtype=dtype)
+            f = _linear(h, lw["wfc1"], bias=lw["bfc1"], act=ops.ACT_GELU)
+            _linear(f, lw["wfc2"], bias=lw["bfc2"], residual=xs, out=xs)
+        return ops.layernorm_fwd(xs, *pk["lnf"], out_dtype=dtype), plan
+
+    @torch.no_grad()
+    def paged_end(self, cache, requests):
+        """The given requests end: their pages, of tokens and frames, go back to the pools."""
+        new = [0] * cache.tokens.requests
+        for r in requests:
+            if not 0 <= int(r) < len(new):
+                raise ValueError(f"no request {r}")
+            new[int(r)] = -1
+        new = torch.tensor(new, dtype=torch.int32, device=cache.bad.device)
+        for part in (cache.tokens, cache.frames):
+            if part is not None:
+                part.plan(new, 1)
+
+    @torch.no_grad()
+    def greedy_ragged(self, prompts, encoder_hidden_states, max_new_tokens, eos_token_id=None, dtype=torch.bfloat16, page_size=64):
+        """Greedy decoding of prompts of different lengths (lists of token ids, none empty) in one ragged batch: each prompt's list with
+        what was generated, up to ``max_new_tokens`` or its own ``eos_token_id``.  A request that is done gives its tokens' pages back in the next step."""
+        R = len(prompts)
+        out = [[int(t) for t in p] for p in prompts]
+        if R == 0 or any(not p for p in out):
+            raise ValueError("greedy_ragged expects prompts of at least one token")
+        dev = encoder_hidden_states.device
+        cache = self.new_paged_cache(R, page_size=page_size, frames=encoder_hidden_states.shape[1], dtype=dtype, device=dev)
+        self.paged_admit(cache, range(R), encoder_hidden_states)
+        most = self.cfg.max_target_positions
+        ids, new, left = [t for p in out for t in p], [len(p) for p in out], [max_new_tokens] * R
+        while any(n > 0 for n in new):
+            h, _ = self.paged_step(cache, torch.tensor(ids, dtype=torch.int64, device=dev), new)
+            live = [r for r in range(R) if new[r] > 0]
+            last = torch.tensor(new, device=dev).clamp_min(0).cumsum(0)[live] - 1
+            nxt = ops.argmax_rows(self.project_tokens(h[last][:, None]).view(len(live), -1)).tolist()
+            ids, new = [], [0] * R
+            for r, t in zip(live, nxt):
+                if left[r] == 0:
+                    new[r] = -1
+                    continue
+                out[r].append(t)
+                left[r] -= 1
+                done = left[r] == 0 or t == eos_token_id or len(out[r]) > most
+                new[r] = -1 if done else 1
+                ids += [] if done else [t]
+        return out
