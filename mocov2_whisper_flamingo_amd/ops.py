@@ -1066,17 +1066,19 @@ def paged_plan(lens, new, table, ring, pool, page_size, max_tokens, *, lens_out=
         raise ValueError("the block table needs a row per request")
     _ints(lens, B, "lens")
     _ints(new, B, "new")
-    _ints(lens_out, B, "lens_out")
     _ints(ring, n, "ring")
     _ints(pool, 2, "pool")
-    _ints(pool_out, 2, "pool_out")
+    if lens_out is not lens:
+        _ints(lens_out, B, "lens_out")
+    if pool_out is not pool:
+        _ints(pool_out, 2, "pool_out")
     stream = _gpu_stream(lens, new, table, ring, pool, lens_out, pool_out)
     lib = _lib.load()
-    buf = torch.empty(B + 2 + 2 * max_tokens, dtype=torch.int32, device=lens.device)
+    buf = lens.new_empty(B + 2 + 2 * max_tokens)
     q_start, slots, positions, status = buf.split_with_sizes((B + 1, max_tokens, max_tokens, 1))
     at = buf.data_ptr()
     ws_bytes = lib.avsr_paged_plan_workspace_bytes(B, max_tokens, n)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=lens.device) if ws_bytes else None
+    ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
     rc = lib.avsr_paged_plan(stream, lens.data_ptr(), new.data_ptr(), table.data_ptr(), ld, width, ring.data_ptr(), n, pool.data_ptr(), B,
                              page_size, max_tokens, lens_out.data_ptr(), pool_out.data_ptr(), at, at + 4 * (B + 1),
                              at + 4 * (B + 1 + max_tokens), at + 4 * (B + 1 + 2 * max_tokens), _p(ws))
@@ -1132,14 +1134,15 @@ def paged_attn(q, k_pages, v_pages, table, lens, q_start, *, max_q=None, max_k=N
     dt = _dt(q)
     stream = _gpu_stream(q, k_pages, v_pages, table, lens, q_start, out)
     if out is None:
-        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+        out, ot, oh = q.new_empty(shape), Hq * D, D
+    else:
+        ot, oh, _ = out.stride()
     if N == 0:
         return out
     lib = _lib.load()
     max_q, max_k = min(N, max_q), min(W * page, max_k)
     ws_bytes = lib.avsr_paged_attn_workspace_bytes(dt, N, B, Hq, Hk, D, max_q, max_k)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    ot, oh, _ = out.stride()
     rc = lib.avsr_paged_attn(stream, dt, q.data_ptr(), qt, qh, k_pages.data_ptr(), kp, kh, v_pages.data_ptr(), vp, vh, table.data_ptr(), ld, W,
                              lens.data_ptr(), q_start.data_ptr(), out.data_ptr(), ot, oh, N, B, Hq, Hk, D, page, n, max_q, max_k, scale,
                              bool(causal), _p(ws), ws_bytes)
@@ -1190,6 +1193,13 @@ def w4_quantize(weight, group=64):
     return w4_pack(q.view(N, G * group)[:, :K].to(torch.int32), scales, group)
 
 
+def _rows(t, M, N, dtype, what):
+    ld, one = t.stride() if t.dim() == 2 else (0, 0)
+    if t.dtype is not dtype or t.shape != (M, N) or one != 1 or (M > 1 and ld < N):
+        raise ValueError(f"{what} must be a row-major [{M}, {N}] tensor of type {dtype}")
+    return ld if M > 1 else N
+
+
 def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=None):
     """act(x @ w^T + bias) + residual for x [M, K] (fp32 or bf16) and a ``W4Weight``: [M, N] of ``out_dtype`` (x's type).
     ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself."""
@@ -1205,26 +1215,24 @@ def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dty
     odt = out_dtype or (x.dtype if out is None else out.dtype)
     if odt not in _DT:
         raise TypeError(f"unsupported dtype {odt}")
-    ldr = N
-    for t, what in ((out, "out"), (residual, "residual")):
-        if t is not None:
-            if t.dtype is not odt or t.shape != (M, N) or t.stride(1) != 1 or (M > 1 and t.stride(0) < N):
-                raise ValueError(f"{what} must be a row-major [{M}, {N}] tensor of type {odt}")
-            ldr = t.stride(0) if M > 1 else N
+    ldr = N if residual is None else _rows(residual, M, N, odt, "residual")
+    ldy = N if out is None else _rows(out, M, N, odt, "out")
     if one != 1 and K > 1 or (M > 1 and ldx < K):
         raise ValueError("x needs unit inner stride")
     if bias is not None and (bias.dtype is not torch.float32 or bias.shape != (N,) or not bias.is_contiguous()):
         raise ValueError(f"bias must be contiguous fp32 [{N}]")
     if act != ACT_NONE and act != ACT_GELU and act != ACT_RELU:
         raise ValueError("act must be ACT_NONE, ACT_GELU or ACT_RELU")
+    if out is not None and out.data_ptr() == x.data_ptr():
+        raise ValueError("out must not be x")
     xdt = _dt(x)
     stream = _gpu_stream(x, packed, scales, bias, residual, out)
     if out is None:
-        out = torch.empty((M, N), dtype=odt, device=x.device)
+        out = x.new_empty((M, N)) if odt is x.dtype else torch.empty((M, N), dtype=odt, device=x.device)
     if M == 0:
         return out
     rc = _lib.load().avsr_w4_matmul(stream, xdt, _DT[odt], x.data_ptr(), ldx if M > 1 else K, packed.data_ptr(), scales.data_ptr(), group,
-                                    _p(bias), act, _p(residual), ldr, out.data_ptr(), out.stride(0) if M > 1 else N, M, N, K)
+                                    _p(bias), act, _p(residual), ldr, out.data_ptr(), ldy, M, N, K)
     check(rc, "avsr_w4_matmul")
     return out
 
