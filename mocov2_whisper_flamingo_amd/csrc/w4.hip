@@ -106,27 +106,36 @@ template <int GS, int MT, int NT> struct W4Wave {
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                f32x4 base = (f32x4){0.f, 0.f, 0.f, 0.f}, acc[NT];
+                // each piece of x has sums of its own: within one, products have 16 bits and hardly any rounding takes place while
+                // the 24 x come and go; the smaller pieces would be rounded at the largest one's 24 x
+                f32x4 base[P], acc[NT][P];
                 bf16x8 xs[GS][P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) base[p] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < GS; ++s)
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
                         xs[s][p] = x(m, q * GS + s, p);
-                        base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus, xs[s][p], base, 0, 0, 0);
+                        base[p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus, xs[s][p], base[p], 0, 0, 0);
                     }
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[n] = base;
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int p = 0; p < P; ++p) acc[n][p] = base[p];
 #pragma unroll
                 for (int s = 0; s < GS; ++s)
 #pragma unroll
                     for (int p = 0; p < P; ++p)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) acc[n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wo[n][s], xs[s][p], acc[n], 0, 0, 0);
+                        for (int n = 0; n < NT; ++n) acc[n][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wo[n][s], xs[s][p], acc[n][p], 0, 0, 0);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) tot[n][m][r] = fmaf(sc[n][r], acc[n][r], tot[n][m][r]);
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = P == 1 ? acc[n][0][r] : acc[n][0][r] + (acc[n][1 % P][r] + acc[n][2 % P][r]);
+                        tot[n][m][r] = fmaf(sc[n][r], v, tot[n][m][r]);
+                    }
             }
         }
     }
