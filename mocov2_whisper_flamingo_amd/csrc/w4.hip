@@ -300,7 +300,8 @@ static int launch_w4(hipStream_t s, W4Args a) {
     const bool wide = a.tiles >= W4_WIDE;
     const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
     if (wide && a.M >= 4) {
-        const int nt = mt == 1 ? 2 : 1, groups = (a.tiles + nt - 1) / nt, rows = a.M < 16 * mt ? a.M : 16 * mt;
+        constexpr int pair = P == 1 ? 2 : 1;                      // two tiles for one read of x, registers permitting
+        const int nt = mt == 1 ? pair : 1, groups = (a.tiles + nt - 1) / nt, rows = a.M < 16 * mt ? a.M : 16 * mt;
         const int most = (W4_X_BYTES / (rows * P) - 16) / 256, blocks = (a.chunks + most - 1) / most;
         a.block = (a.chunks + blocks - 1) / blocks;              // blocks of one size
         a.kw = 1;
@@ -309,7 +310,7 @@ static int launch_w4(hipStream_t s, W4Args a) {
         const int tw = W4_WAVES / a.kw;
         const dim3 grid((groups + tw - 1) / tw, (a.M + 16 * mt - 1) / (16 * mt)), block(64 * W4_WAVES);
 #define L(MT, NT) hipLaunchKernelGGL((w4_staged_kernel<TX, GS, MT, NT>), grid, block, lds, s, a)
-        if (mt == 1) L(1, 2); else if (mt == 2) L(2, 1); else L(4, 1);
+        if (mt == 1) L(1, pair); else if (mt == 2) L(2, 1); else L(4, 1);
 #undef L
         return avsr_launch_status();
     }

@@ -368,6 +368,14 @@ def test_w4_wide(dev, xt, M, N, K):
     w4_check(dev, M, N, K, 64, xt, F32)
 
 
+@pytest.mark.parametrize("xt,ot", [(BF, BF), (F32, F32)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K,pad", [(3, 16400, 200, 0), (5, 16385, 1000, 0), (16, 16400, 333, 5), (4, 16384, 4480, 0), (33, 16390, 1160, 0), (70, 16384, 130, 0)])
+def test_w4_wide_through_lds(dev, xt, ot, group, M, N, K, pad):
+    """Wide layers: x in one block and in several, rows that are not aligned, more rows than a workgroup takes."""
+    w4_check(dev, M, N, K, group, xt, ot, pad=pad, residual=bool(pad), act=ops.ACT_GELU if pad else ops.ACT_NONE)
+
+
 @pytest.mark.parametrize("act", [ops.ACT_NONE, ops.ACT_GELU, ops.ACT_RELU])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("xt,ot", [(BF, BF), (BF, F32), (F32, F32)])
