@@ -1072,6 +1072,8 @@ def paged_plan(lens, new, table, ring, pool, page_size, max_tokens, *, lens_out=
         _ints(lens_out, B, "lens_out")
     if pool_out is not pool:
         _ints(pool_out, 2, "pool_out")
+    if new.data_ptr() == lens_out.data_ptr():
+        raise ValueError("new must not be the lengths")
     stream = _gpu_stream(lens, new, table, ring, pool, lens_out, pool_out)
     lib = _lib.load()
     buf = lens.new_empty(B + 2 + 2 * max_tokens)
