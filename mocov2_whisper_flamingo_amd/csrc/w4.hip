@@ -193,7 +193,9 @@ template <int GS, int MT, int NT> struct W4Wave {
     }
 };
 
-// ---- x straight from L2: nothing to wait for before the first product.  The waves of a workgroup take the 128-column
+// ---- x straight from L2: nothing to wait for before the first product.  1x16384x8192 (69 MB) takes 16 us, 4.3 TB/s, of
+// which 12 are the bytes at the rate of a long read; a layer of a small decoder (1x1152x384) 3.5 us, a launch and two trips
+// to memory.  The waves of a workgroup take the 128-column
 // chunks in turn.  A chunk's weights and scales (AHEAD: its x too) are loaded while the one before is multiplied.  Rows of x
 // behind the last are read as the last one: their columns of the product are never stored.
 #define W4_WAVES 8
@@ -246,10 +248,11 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_direct_kernel(W4Args a) {
     ww.finish(a, sums, t0, m0, wave, wave, waves, lane);
 }
 
-// ---- x through LDS, for wide layers: read by every wave for its own columns it takes up the vector memory path longer than
+// ---- x through LDS, for wide layers and more than a few rows: read by every wave for its own columns it takes up the vector memory path longer than
 // the weights do (16 rows: 4 KiB against 1 KiB a tile), here eight waves share it, and fp32 is taken apart once.  The waves
 // are kw ways of the chunks times 8 / kw groups of weight tiles.  x is staged in blocks of chunks, as many as fit, a row 16
-// bytes longer than its values so that the 16 rows a fragment reads lie in different banks.
+// bytes longer than its values so that the 16 rows a fragment reads lie in different banks.  16x51865x1280 14 us (39 MB; 7 at
+// the rate of a long read, the rest is filling the pipeline: a wave has five chunks), 64x51865x768 25 us (direct 40).
 template <typename TX, int GS, int MT, int NT>
 __global__ __launch_bounds__(64 * W4_WAVES, XFrag<TX>::P == 1 || MT < 4 ? 4 : 2) void w4_staged_kernel(W4Args a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -292,14 +295,15 @@ __global__ __launch_bounds__(64 * W4_WAVES, XFrag<TX>::P == 1 || MT < 4 ? 4 : 2)
 }
 
 #define W4_FILL 4096            // waves that the chip is given: 16 per CU
-#define W4_WIDE 1024            // tiles of weight rows from which a wave takes two (enough waves all the same)
+#define W4_WIDE 1024            // tiles of weight rows (16384 rows) from which a wave takes two: 32768 rows for 4 8.7 us (one: 9.9), 12288 rows 6.1 (5.6)
+#define W4_STAGED 8             // rows of x above which a wide layer takes it through LDS: 51865x1280 for 16 14.1 us (direct 16.7), for 4 9.0 (8.7)
 #define W4_X_BYTES 65536        // x in LDS: two workgroups share a CU
 template <typename TX, int GS>
 static int launch_w4(hipStream_t s, W4Args a) {
     constexpr int P = XFrag<TX>::P;
     const bool wide = a.tiles >= W4_WIDE;
     const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    if (wide && a.M >= 4) {
+    if (wide && a.M > W4_STAGED) {
         constexpr int pair = P == 1 ? 2 : 1;                      // two tiles for one read of x, registers permitting
         const int nt = mt == 1 ? pair : 1, groups = (a.tiles + nt - 1) / nt, rows = a.M < 16 * mt ? a.M : 16 * mt;
         const int most = (W4_X_BYTES / (rows * P) - 16) / 256, blocks = (a.chunks + most - 1) / most;
