@@ -693,7 +693,7 @@ template <int D> __device__ __forceinline__ void store_vals(float* p, const floa
 // 85 us, 5.8 TB/s, the rate of a long read; 4 requests of 7000 to 32700 keys, 8 heads of 128 (271 MB), 56 us and 5 for the
 // join; 8 requests x 6 heads x 440 keys 7 us, a launch and three dependent trips to memory.
 template <typename T, int D, int WAVES, bool AHEAD>
-__global__ __launch_bounds__(64 * WAVES, sizeof(T) * D <= 128 ? (AHEAD ? 3 : 4) : 2) void paged_attn_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? 2 : sizeof(T) == 4 || AHEAD ? 3 : 4) void paged_attn_few_kernel(AttnArgs a) {
     typedef Frag<T, D> F;
     __shared__ float s_m[WAVES][16], s_l[WAVES][16];
     __shared__ float s_o[WAVES][16][D + 4];
@@ -1199,10 +1199,13 @@ static AttnPlan attn_plan(int dtype, int64_t D, int64_t N, int64_t B, int64_t Hk
     const int64_t fill = (p.chunk ? 512 : bytes <= 128 ? 768 : 1536) / wgs, most = p.chunk ? (max_k + 255) / 256 : max_k <= 512 ? 1 : (max_k + 127) / 128;
     const int64_t s = fill < most ? fill : most;
     p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-    // eight waves where the workgroups leave CUs free; the next tile ahead of time where there is a long way to go (64 requests
-    // x 20 heads: 1500 keys 91 -> 85 us with it, 20 to 440 keys 14.1 -> 16 us: fewer waves fit) and registers for it
+    // Eight waves where the workgroups leave CUs free.  The next tile ahead of time where a wave has a long way to go (64
+    // requests x 20 heads of 1500 keys 91 -> 85 us) or all workgroups run at once anyway (40 requests x 8 heads of 60 to 448 keys
+    // 11.2 -> 10.2 us); with more and short ones, more waves are better (64 x 20 of 20 to 440 keys 14.1 us, 16 ahead).  Only 128
+    // bytes a key leave registers for it.
+    const int64_t rows_tiles = B * p.tiles_few < N * G / 16 + B ? B * p.tiles_few : N * G / 16 + B;
     p.waves = p.few && wgs * p.splits <= 256 ? 8 : 4;
-    p.ahead = bytes <= 128 && (p.waves == 8 || max_k > 512);
+    p.ahead = bytes <= 128 && (p.waves == 8 || max_k > 512 || rows_tiles * Hk * p.splits <= 768);
     p.grid_few = p.few ? B * Hk * p.splits : 0;
     p.grid_chunk = Hk * p.chunk_tiles * p.splits;
     p.floats = p.splits > 1 ? N * Hk * G * p.splits * (D + 2) : 0;
