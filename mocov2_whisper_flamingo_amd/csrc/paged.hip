@@ -314,6 +314,10 @@ extern "C" int avsr_paged_write(avsr_stream_t stream, int in_dtype, int page_dty
     const int shift = page_shift(page);
     if (shift < 0 || (head_dim != 64 && head_dim != 128) || n_pages > (1LL << (30 - shift)) || H > (1 << 16)) return AVSR_EUNSUPPORTED;
     const int64_t qi = in_dtype == AVSR_F32 ? 4 : 8, qo = page_dtype == AVSR_F32 ? 4 : 8;
+    // the stride of a dimension of one is never used
+    if (rows <= 1) ldk = ldv = 0;
+    if (H == 1) k_head = v_head = k_head_stride = v_head_stride = 0;
+    if (n_pages == 1) k_page_stride = v_page_stride = 0;
     if ((ldk | ldv | k_head | v_head) % qi || (k_page_stride | k_head_stride | v_page_stride | v_head_stride) % qo ||
         ((uintptr_t)k | (uintptr_t)v | (uintptr_t)k_pages | (uintptr_t)v_pages) % 16) return AVSR_EUNSUPPORTED;
     if (rows == 0) return AVSR_OK;
@@ -1246,6 +1250,10 @@ extern "C" int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, i
     const int shift = page_shift(page);
     if (shift < 0 || (head_dim != 64 && head_dim != 128) || n_pages > (1LL << (30 - shift)) || width > (1LL << (30 - shift))) return AVSR_EUNSUPPORTED;
     const int64_t qm = dtype == AVSR_F32 ? 4 : 8;
+    if (N <= 1) ldq = ldo = 0;                                  // the stride of a dimension of one is never used
+    if (Hq == 1) q_head = o_head = 0;
+    if (Hk == 1) k_head_stride = v_head_stride = 0;
+    if (n_pages == 1) k_page_stride = v_page_stride = 0;
     if ((ldq | q_head | k_page_stride | k_head_stride | v_page_stride | v_head_stride | ldo | o_head) % qm ||
         ((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o) % 16) return AVSR_EUNSUPPORTED;
     if (N > (1 << 28) || N * Hq > (1LL << 30) || B > (1 << 24) || B * Hk > (1LL << 24)) return AVSR_EUNSUPPORTED;

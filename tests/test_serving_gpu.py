@@ -133,6 +133,24 @@ def test_write_takes_heads_of_any_stride(dev):
     assert torch.equal(kp[1, :, 15], rows[0]) and torch.equal(vp[0, :, 0], rows[1]) and torch.equal(kp[0, :, 5], rows[2]) and x.shape[0] == 3
 
 
+def test_strides_of_a_dimension_of_one_do_not_count(dev):
+    """Views of one row, one head or one page whose stride there is any number: PyTorch leaves it free."""
+    def odd(x):
+        return x.as_strided(x.shape, [13 if n == 1 else s for n, s in zip(x.shape, x.stride())])
+
+    g = torch.Generator().manual_seed(1)
+    for shape in ((1, 3), (4, 1), (1, 1)):
+        k = torch.randn(*shape, 64, generator=g).to(BF).to(dev)
+        slots = i32(list(range(shape[0])), dev)
+        a, b = torch.zeros(2, 1, shape[1], 16, 64, dtype=BF, device=dev), torch.zeros(2, 1, shape[1], 16, 64, dtype=BF, device=dev)
+        ops.paged_write(k, k, a[0], a[1], slots)
+        ops.paged_write(odd(k), odd(k), odd(b[0]), odd(b[1]), slots)
+        assert torch.equal(a, b) and a.any()
+        tail = (i32([[0]], dev), i32([shape[0]], dev), i32([0, shape[0]], dev))
+        want = ops.paged_attn(k, a[0], a[1], *tail, scale=0.125)
+        assert torch.equal(ops.paged_attn(odd(k), odd(a[0]), odd(a[1]), *tail, scale=0.125, out=odd(torch.zeros_like(k))), want)
+
+
 # ------------------------------------------------------------- attention ----
 def attend_and_check(dev, lens, news, Hq, Hk, D, page, dtype, causal, *, seed=0, layout="heads", scale=None, edit=None, **kw):
     g = torch.Generator().manual_seed(seed)
