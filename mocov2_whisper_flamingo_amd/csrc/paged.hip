@@ -1247,6 +1247,7 @@ extern "C" int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, i
     if (!q || !k_pages || !v_pages || !table || !lens || !q_start || !o) return AVSR_EINVAL;
     if (N < 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk || width <= 0 || ld_table < width || n_pages <= 0 || max_q <= 0 || max_k <= 0) return AVSR_EINVAL;
     if (dtype != AVSR_F32 && dtype != AVSR_BF16) return AVSR_EINVAL;
+    if (!(fabsf(scale * LOG2E) < INFINITY)) return AVSR_EINVAL;
     const int shift = page_shift(page);
     if (shift < 0 || (head_dim != 64 && head_dim != 128) || n_pages > (1LL << (30 - shift)) || width > (1LL << (30 - shift))) return AVSR_EUNSUPPORTED;
     const int64_t qm = dtype == AVSR_F32 ? 4 : 8;

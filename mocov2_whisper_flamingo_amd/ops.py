@@ -1133,6 +1133,8 @@ def paged_attn(q, k_pages, v_pages, table, lens, q_start, *, max_q=None, max_k=N
     max_k = W * page if max_k is None else int(max_k)
     if (N and max_q < 1) or max_k < 1:
         raise ValueError("max_q and max_k must be positive")
+    if not abs(scale) < 1e38:
+        raise ValueError("scale must be a finite number")
     dt = _dt(q)
     stream = _gpu_stream(q, k_pages, v_pages, table, lens, q_start, out)
     if out is None:

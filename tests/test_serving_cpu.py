@@ -78,6 +78,16 @@ def test_attn_refuses(change):
         ops.paged_attn(**a)
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_attn_refuses_a_scale_that_is_not_finite(scale):
+    pages = z(4, 2, 16, 64, dtype=torch.float32)
+    with pytest.raises(ValueError):
+        ops.paged_attn(z(3, 2, 64, dtype=torch.float32), pages, pages, z(2, 3), z(2), z(3), scale=scale)
+    p = 4096
+    assert _lib.load().avsr_paged_attn(None, 1, p, 256, 64, p, 4096, 1024, p, 4096, 1024, p, 3, 3, p, p, p, 256, 64, 3, 2, 4, 2, 64, 16, 9, 1, 40,
+                                       scale, 1, None, 0) == -1
+
+
 def test_w4_refuses():
     w = ops.w4_pack(z(5, 40), torch.ones(5, 2), 32)
     x = z(2, 40, dtype=torch.float32)
