@@ -1167,6 +1167,8 @@ def w4_pack(q, scales, group):
         raise ValueError("w4_pack expects whole numbers [N, K] and scales [N, ceil(K / group)]")
     if int(q.min()) < -8 or int(q.max()) > 7:
         raise ValueError("4-bit weights lie in -8 .. 7")
+    if not bool(torch.isfinite(scales).all()):
+        raise ValueError("scales must be finite")
     N, K = q.shape
     T, C = -(-N // 16), -(-K // 128)
     full = torch.zeros((T * 16, C * 128), dtype=torch.int32, device=q.device)
@@ -1188,6 +1190,8 @@ def w4_quantize(weight, group=64):
     if weight.dim() != 2 or 0 in weight.shape or not weight.dtype.is_floating_point:
         raise ValueError("w4_quantize expects a floating-point [N, K] weight")
     w = weight.detach().float()
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("weights must be finite")
     N, K = w.shape
     G = -(-K // group)
     w = torch.nn.functional.pad(w, (0, G * group - K)).view(N, G, group)

@@ -103,6 +103,16 @@ def test_w4_refuses():
             call()
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_w4_weights_and_scales_have_to_be_finite(bad):
+    w = torch.ones(3, 40)
+    w[1, 7] = bad
+    with pytest.raises(ValueError, match="finite"):
+        ops.w4_quantize(w, 32)
+    with pytest.raises(ValueError, match="finite"):
+        ops.w4_pack(z(3, 40), w[:, 6:8], 32)
+
+
 def test_c_entries_refuse_before_they_launch():
     """Status codes of calls whose pointers are never read: -1 for what cannot be, -2 for what is not built."""
     lib = _lib.load()
