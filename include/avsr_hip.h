@@ -595,7 +595,8 @@ int avsr_embed_tokens_at(avsr_stream_t stream, int table_dtype, const int64_t* i
  * word[n/16][k/128][k/8 % 4][n % 16][k/32 % 4], the nibble of k % 8 = e at bit 4*(e/2) + 16*(e%2); scales: bf16
  * [n/16][k/group][n % 16]; both padded to whole tiles of 16 rows and 128 columns with nibble 8 and scale 0.
  * group: 32, 64 or 128.  x fp32 or bf16, y and residual fp32 or bf16 (residual of y's type, may be y itself); act NONE,
- * GELU or RELU.  fp32 sums.  A row of x with a value that is not finite yields NaN. */
+ * GELU or RELU.  fp32 sums, which pass through some thousand times the largest x: it is at most 1e34 in magnitude.  A row
+ * of x with a value that is not finite yields NaN. */
 int avsr_w4_matmul(avsr_stream_t stream, int x_dtype, int out_dtype, const void* x, int64_t ldx, const void* packed,
                    const void* scales, int64_t group, const float* bias, int act, const void* residual, int64_t ldr,
                    void* y, int64_t ldy, int64_t M, int64_t N, int64_t K);

@@ -1210,7 +1210,8 @@ def _rows(t, M, N, dtype, what):
 
 def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=None):
     """act(x @ w^T + bias) + residual for x [M, K] (fp32 or bf16) and a ``W4Weight``: [M, N] of ``out_dtype`` (x's type).
-    ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself."""
+    ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself.  x is at most 1e34 in
+    magnitude: a sum passes through some thousand times that, and a row of x with an infinity or NaN is NaN throughout."""
     packed, scales, N, K, group = w
     T, C = (N + 15) // 16, (K + 127) // 128
     if (group not in W4_GROUPS or packed.dtype is not torch.int32 or packed.numel() != T * C * 256 or scales.dtype is not torch.bfloat16
@@ -1231,7 +1232,7 @@ def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dty
         raise ValueError(f"bias must be contiguous fp32 [{N}]")
     if act != ACT_NONE and act != ACT_GELU and act != ACT_RELU:
         raise ValueError("act must be ACT_NONE, ACT_GELU or ACT_RELU")
-    if out is not None and out.data_ptr() == x.data_ptr():
+    if out is not None and M and out.data_ptr() == x.data_ptr():
         raise ValueError("out must not be x")
     xdt = _dt(x)
     stream = _gpu_stream(x, packed, scales, bias, residual, out)

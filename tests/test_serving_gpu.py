@@ -410,6 +410,17 @@ def test_w4_adds_onto_its_own_output(dev):
     assert torch.equal(ops.w4_matmul(x, w, residual=y, out=y), want) and torch.equal(y, want)
 
 
+@pytest.mark.parametrize("xt", [BF, F32])
+def test_w4_no_rows_and_large_values(dev, xt):
+    """No rows, also into a given output; and the largest values allowed, whose sums on the way stay finite."""
+    w = ops.w4_pack(torch.full((20, 256), -8, dtype=torch.int32), torch.full((20, 2), 2.0 ** -10), 128)
+    w = w._replace(packed=w.packed.to(dev), scales=w.scales.to(dev))
+    x = torch.full((1, 256), 2.0 ** 112, dtype=xt, device=dev)                       # 5.2e33
+    none = ops.w4_matmul(x[:0], w, out=torch.empty(0, 20, dtype=xt, device=dev), residual=torch.empty(0, 20, dtype=xt, device=dev))
+    assert none.shape == (0, 20) and ops.w4_matmul(x[:0], w).shape == (0, 20)
+    assert torch.equal(ops.w4_matmul(x, w).cpu(), torch.full((1, 20), -(2.0 ** 113), dtype=xt))         # 256 * 2^112 * -8 * 2^-10
+
+
 def test_w4_rows_do_not_mix(dev):
     """A row that is not finite is NaN throughout and leaves the others alone, and a row's result does not depend on how many
     rows stand beside it in its tile."""
