@@ -276,12 +276,14 @@ class WhisperDecoder(nn.Module):
 
     @torch.no_grad()
     def paged_admit(self, cache, requests, encoder_hidden_states):
-        """Encoder output [n, Te, D] of the n given requests (ascending, none of which holds frames) into the cache's frames.  Raises if
-        the pages do not suffice, with nothing changed."""
+        """Encoder output [n, Te, D] of the n given requests (ascending, none of which holds frames) into the cache's frames.  Raises
+        with nothing changed on what does not fit: its width, its device, or the free pages."""
         if cache.frames is None:
             raise ValueError("the cache was made without frames")
         requests = [int(r) for r in requests]
         n, Te, D = encoder_hidden_states.shape
+        if D != self.cfg.d_model or encoder_hidden_states.device != cache.bad.device or Te == 0:
+            raise ValueError(f"paged_admit expects encoder output [n, frames, {self.cfg.d_model}] on the cache's device")
         if len(requests) != n or n == 0 or any(b <= a for a, b in zip(requests, requests[1:])) or requests[0] < 0 or requests[-1] >= cache.frames.requests:
             raise ValueError("paged_admit expects one ascending request index per encoder output")
         if bool((cache.frames.lens[requests] != 0).any()):
@@ -289,10 +291,11 @@ class WhisperDecoder(nn.Module):
         new = [0] * cache.frames.requests
         for r in requests:
             new[r] = Te
+        kvs = self.cross_kv(encoder_hidden_states, cache.dtype)      # what can fail here comes before the pages are taken
         plan = cache.frames.plan(torch.tensor(new, dtype=torch.int32, device=cache.bad.device), n * Te)
         cache.frames.check(plan)
         H = self.cfg.decoder_attention_heads
-        for i, kv in enumerate(self.cross_kv(encoder_hidden_states, cache.dtype)):
+        for i, kv in enumerate(kvs):
             kv = kv.view(n * Te, 2 * D)
             cache.frames.write(i, kv[:, :D].unflatten(1, (H, -1)), kv[:, D:].unflatten(1, (H, -1)), plan)
 

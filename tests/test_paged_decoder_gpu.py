@@ -130,6 +130,20 @@ def test_a_step_that_does_not_fit_changes_nothing(dev):
         PagedKVCache(1, 1, 1, pages=0, max_tokens=16)
 
 
+def test_frames_that_cannot_be_admitted_take_no_pages(dev):
+    """Encoder output of another width, on another device, or without frames."""
+    dec, sd, cfg = model(dev)
+    cache = dec.new_paged_cache(2, frames=32, page_size=16)
+    for bad in (torch.zeros(1, 8, cfg.d_model + 8, device=dev), torch.zeros(1, 8, cfg.d_model), torch.zeros(1, 0, cfg.d_model, device=dev)):
+        with pytest.raises(ValueError):
+            dec.paged_admit(cache, [0], bad)
+    with pytest.raises(_lib.AvsrHipError, match="outgrows"):
+        dec.paged_admit(cache, [0], torch.zeros(1, 33, cfg.d_model, device=dev))
+    assert cache.frames.lens.tolist() == [0, 0] and cache.frames.pool.tolist() == [0, 4]
+    dec.paged_admit(cache, [0, 1], torch.zeros(2, 32, cfg.d_model, device=dev))
+    assert cache.frames.pool.tolist() == [0, 0]
+
+
 def test_greedy_ragged_is_greedy_for_each_prompt(dev):
     dec, sd, cfg = model(dev, seed=23)
     g = torch.Generator().manual_seed(5)
