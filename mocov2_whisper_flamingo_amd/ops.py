@@ -1117,7 +1117,7 @@ def paged_attn(q, k_pages, v_pages, table, lens, q_start, *, max_q=None, max_k=N
     q_start[b+1]-1 are the last tokens of request b, ``lens`` [B] counts its tokens with them; ``causal=False``: each row sees all
     of them (cross-attention).  Hq is a multiple of the pages' heads.  ``max_q`` / ``max_k``: at most so many new tokens / keys in a
     request - they choose how the work is split, larger requests still come out right.  Rows behind the last request are left as
-    they are."""
+    they are.  ``out`` may be q."""
     n, Hk, page, D, kp, kh, vp, vh = _pages(k_pages, v_pages)
     shape = q.shape
     if len(shape) != 3 or shape[2] != D or shape[1] == 0 or shape[1] % Hk or q.dtype is not k_pages.dtype:

@@ -214,6 +214,60 @@ def test_attn_chunks(dev, dtype, D, page, causal):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B", [64, 65, 150])
+@pytest.mark.parametrize("causal", [True, False])
+def test_attn_chunks_of_many_requests(dev, dtype, D, B, causal):
+    """Around 64 requests the tiles are dealt out in another way: prompts on both sides of a tile's 128 rows (64 tokens of two
+    heads), single tokens and requests that wait between them."""
+    rng = random.Random(B + D)
+    news = [rng.choice([0, 0, 1, 1, 2, 31, 33, 63, 64, 65, 130]) for _ in range(B)]
+    news[0], news[-1] = 65, 129
+    lens = [n + rng.choice([0, 0, 5, 64, 190]) for n in news]
+    attend_and_check(dev, lens, news, 2, 1, D, 32, dtype, causal, seed=B)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lens,news", [([40, 300, 7], [1, 1, 1]), ([300, 200, 64, 3], [130, 70, 1, 3]), ([9000], [1])])
+def test_attn_into_its_own_queries(dev, dtype, lens, news):
+    """out may be q: a row's queries are read before its result is written, in each kernel, whole and split."""
+    g = torch.Generator().manual_seed(8)
+    start = [0]
+    for n in news:
+        start.append(start[-1] + n)
+    c = Cache(lens, 2, 64, 64, dtype, g)
+    kp, vp = c.views(dev)
+    q = torch.randn(start[-1], 4, 64, generator=g).to(dtype).to(dev)
+    tail = (kp, vp, c.table.to(dev), i32(lens, dev), i32(start, dev))
+    want = ops.paged_attn(q, *tail, scale=0.125)
+    assert torch.equal(ops.paged_attn(q, *tail, scale=0.125, out=q), want) and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("news", [[3, 2], [70, 90], [200, 40]])
+@pytest.mark.parametrize("G", [1, 3])
+def test_attn_values_that_are_not_finite_inside_a_chunk(dev, dtype, D, news, G):
+    """An infinite value in the middle of the new tokens: rows before it are as without it, rows from it on are infinite in its column."""
+    g = torch.Generator().manual_seed(9)
+    lens = [n + 37 for n in news]
+    c = Cache(lens, 2, D, 16, dtype, g)
+    kp, vp = c.views(dev)
+    q = torch.randn(sum(news), 2 * G, D, generator=g).to(dtype)
+    hit = [37 + n // 2 for n in news]
+    for b in range(2):
+        vp[c.table[b, hit[b] // 16].item(), 1, hit[b] % 16, 5] = float("inf")
+    got = ops.paged_attn(q.to(dev), kp, vp, c.table.to(dev), i32(lens, dev), i32([0, news[0], sum(news)], dev), scale=D ** -0.5).cpu()
+    for b in range(2):
+        rows = got[sum(news[:b]):sum(news[:b + 1])].double()
+        o, bound = attn_ref(q[sum(news[:b]):sum(news[:b + 1])], c.k[b], c.v[b], D ** -0.5, True, dtype)
+        seen = torch.zeros_like(rows, dtype=torch.bool)
+        seen[hit[b] - 37:, G:, 5] = True
+        assert torch.isinf(rows[seen]).all() and (rows[seen] > 0).all()
+        assert ((rows - o).abs() <= bound)[~seen].all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 def test_attn_one_request(dev, dtype):
     attend_and_check(dev, [200], [200], 2, 1, 64, 16, dtype, True)
     attend_and_check(dev, [33], [33], 1, 1, 64, 16, dtype, True)
