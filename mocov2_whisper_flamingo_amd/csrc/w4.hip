@@ -195,39 +195,32 @@ template <int GS, int MT, int NT> struct W4Wave {
 
 // ---- x straight from L2: nothing to wait for before the first product.  1x16384x8192 (69 MB) takes 16 us, 4.3 TB/s, of
 // which 12 are the bytes at the rate of a long read; a layer of a small decoder (1x1152x384) 3.5 us, a launch and two trips
-// to memory.  The waves of a workgroup take the 128-column
-// chunks in turn.  A chunk's weights and scales (AHEAD: its x too) are loaded while the one before is multiplied.  Rows of x
-// behind the last are read as the last one: their columns of the product are never stored.
+// to memory.  Up to 16 rows.  The waves of a workgroup take the 128-column chunks in turn.  A chunk's weights and scales
+// (AHEAD: its x too) are loaded while the one before is multiplied.  Rows of x behind the last are read as the last one: their
+// columns of the product are never stored.
 #define W4_WAVES 8
-template <typename TX, int GS, int MT, int NT, bool AHEAD>
+template <typename TX, int GS, int NT, bool AHEAD>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_direct_kernel(W4Args a) {
     extern __shared__ f32x4 sums[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int t0 = blockIdx.x * NT, m0 = blockIdx.y * 16 * MT, g = lane >> 4;
-    W4Wave<GS, MT, NT> ww(a, t0, lane);
-    const TX* xp[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) xp[m] = (const TX*)a.x + (long)min(m0 + 16 * m + (lane & 15), a.M - 1) * a.ldx + 8 * g;
-    struct X { XFrag<TX> x[MT][4]; };
+    const int t0 = blockIdx.x * NT, g = lane >> 4;
+    W4Wave<GS, 1, NT> ww(a, t0, lane);
+    const TX* xp = (const TX*)a.x + (long)min(lane & 15, a.M - 1) * a.ldx + 8 * g;
+    struct X { XFrag<TX> x[4]; };
     const int whole = a.vec_x ? a.K >> 7 : 0;                     // chunks whose x can be read in 16-byte pieces
     auto load_x = [&](X& st, int c) {
-        if (c < whole) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) st.x[m][s].load(xp[m] + c * 128 + 32 * s);
-        } else {
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int s = 0; s < 4; ++s) st.x[m][s].load(xp[m] + c * 128 + 32 * s, a.K - (c * 128 + 32 * s + 8 * g));
+        for (int s = 0; s < 4; ++s) {
+            const int k = c * 128 + 32 * s;
+            if (c < whole) st.x[s].load(xp + k);
+            else st.x[s].load(xp + k, a.K - (k + 8 * g));
         }
     };
-    typename W4Wave<GS, MT, NT>::W sw[2];
+    typename W4Wave<GS, 1, NT>::W sw[2];
     X sx[AHEAD ? 2 : 1];
     auto add = [&](int u) {
         const X& x = sx[AHEAD ? u : 0];
-        ww.template add<XFrag<TX>::P>(sw[u], [&](int m, int s, int p) { return x.x[m][s].piece(p); });
+        ww.template add<XFrag<TX>::P>(sw[u], [&](int, int s, int p) { return x.x[s].piece(p); });
     };
     // loads come back in order: x of a chunk is asked for before weights that are further ahead
     if (AHEAD && wave < a.chunks) load_x(sx[0], wave);
@@ -245,16 +238,18 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_direct_kernel(W4Args a) {
             add(u);
         }
     }
-    ww.finish(a, sums, t0, m0, wave, wave, waves, lane);
+    ww.finish(a, sums, t0, 0, wave, wave, waves, lane);
 }
 
-// ---- x through LDS, for wide layers and more than a few rows: read by every wave for its own columns it takes up the vector memory path longer than
-// the weights do (16 rows: 4 KiB against 1 KiB a tile), here eight waves share it, and fp32 is taken apart once.  The waves
-// are kw ways of the chunks times 8 / kw groups of weight tiles.  x is staged in blocks of chunks, as many as fit, a row 16
-// bytes longer than its values so that the 16 rows a fragment reads lie in different banks.  16x51865x1280 14 us (39 MB; 7 at
-// the rate of a long read, the rest is filling the pipeline: a wave has five chunks), 64x51865x768 25 us (direct 40).
+// ---- x through LDS, for more than a few rows.  A fragment of x is 16 rows: read from L2 it touches 16 cache lines per quarter of a
+// wave, 64 lines for the 1 KiB of weights it is multiplied with, and every wave does so for its own columns.  Here eight waves
+// share x, whose rows are read in order, and fp32 is taken apart once.  The waves are kw ways of the chunks times 8 / kw groups
+// of weight tiles.  x is staged in blocks of chunks, as many as fit, a row 16 bytes longer than its values so that the 16 rows a
+// fragment reads lie in different banks.  16x51865x1280 14 us (39 MB; 7 at the rate of a long read, the rest is filling the
+// pipeline: a wave has ten chunks), 64x51865x768 22 us (direct 40), 64x5120x1280 7.9 us (direct 14.7; 3.3 MB of weights: staging x
+// and two barriers are most of it), 64x8192x8192 35 us.
 template <typename TX, int GS, int MT, int NT>
-__global__ __launch_bounds__(64 * W4_WAVES, XFrag<TX>::P == 1 || MT < 4 ? 4 : 2) void w4_staged_kernel(W4Args a) {
+__global__ __launch_bounds__(64 * W4_WAVES, 4) void w4_staged_kernel(W4Args a) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     constexpr int P = XFrag<TX>::P;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -270,14 +265,26 @@ __global__ __launch_bounds__(64 * W4_WAVES, XFrag<TX>::P == 1 || MT < 4 ? 4 : 2)
         if (first < b1) ww.load(sw[0], first);
         if (b0) __syncthreads();                                 // the block before has been read
         const int pieces = (b1 - b0) * 16;                       // of eight values, of a row
-        for (int j = threadIdx.x; j < rows * pieces; j += 64 * W4_WAVES) {
-            const int row = j / pieces, pc = j - row * pieces, k = b0 * 128 + pc * 8;
-            const TX* x = (const TX*)a.x + (long)(m0 + row) * a.ldx + (k < a.K ? k : 0);
-            XFrag<TX> f;
-            if (a.vec_x && k + 8 <= a.K) f.load(x);
-            else f.load(x, a.K - k);
+        constexpr int U = P * MT == 1 ? 4 : 2;                   // pieces in flight per thread
+        for (int j0 = threadIdx.x; j0 < rows * pieces; j0 += U * 64 * W4_WAVES) {
+            XFrag<TX> f[U];
 #pragma unroll
-            for (int p = 0; p < P; ++p) *(bf16x8*)(lds + (p * rows + row) * stride + pc * 16) = f.piece(p);
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * 64 * W4_WAVES;
+                if (j >= rows * pieces) break;
+                const int row = j / pieces, k = b0 * 128 + (j - row * pieces) * 8;
+                const TX* x = (const TX*)a.x + (long)(m0 + row) * a.ldx + (k < a.K ? k : 0);
+                if (a.vec_x && k + 8 <= a.K) f[u].load(x);
+                else f[u].load(x, a.K - k);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int j = j0 + u * 64 * W4_WAVES;
+                if (j >= rows * pieces) break;
+                const int row = j / pieces;
+#pragma unroll
+                for (int p = 0; p < P; ++p) *(bf16x8*)(lds + (p * rows + row) * stride + (j - row * pieces) * 16) = f[u].piece(p);
+            }
         }
         __syncthreads();
         for (int c0 = first; c0 < b1; c0 += 2 * a.kw) {
@@ -296,40 +303,53 @@ __global__ __launch_bounds__(64 * W4_WAVES, XFrag<TX>::P == 1 || MT < 4 ? 4 : 2)
 
 #define W4_FILL 4096            // waves that the chip is given: 16 per CU
 #define W4_WIDE 1024            // tiles of weight rows (16384 rows) from which a wave takes two: 32768 rows for 4 8.7 us (one: 9.9), 12288 rows 6.1 (5.6)
-#define W4_STAGED 8             // rows of x above which a wide layer takes it through LDS: 51865x1280 for 16 14.1 us (direct 16.7), for 4 9.0 (8.7)
-#define W4_X_BYTES 65536        // x in LDS: two workgroups share a CU
+#define W4_GROUPS 144           // workgroups of the staged kernel, at least: each of them reads all its rows of x, so not many more either
+#define W4_X_BYTES 65536        // x in LDS where two workgroups share a CU; twice that where each has one to itself
 template <typename TX, int GS>
 static int launch_w4(hipStream_t s, W4Args a) {
-    constexpr int P = XFrag<TX>::P;
+    constexpr int P = XFrag<TX>::P, PAIR = P == 1 ? 2 : 1;        // two tiles for one read of x, registers permitting
     const bool wide = a.tiles >= W4_WIDE;
-    const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    if (wide && a.M > W4_STAGED) {
-        constexpr int pair = P == 1 ? 2 : 1;                      // two tiles for one read of x, registers permitting
-        const int nt = mt == 1 ? pair : 1, groups = (a.tiles + nt - 1) / nt, rows = a.M < 16 * mt ? a.M : 16 * mt;
-        const int most = (W4_X_BYTES / (rows * P) - 16) / 256, blocks = (a.chunks + most - 1) / most;
-        a.block = (a.chunks + blocks - 1) / blocks;              // blocks of one size
-        a.kw = 1;
-        while (a.kw < W4_WAVES && groups * a.kw * 2 <= W4_FILL && a.kw < a.block) a.kw *= 2;
-        const int xb = rows * P * (a.block * 256 + 16), sb = a.kw > 1 ? W4_WAVES * nt * mt * 1024 : 0, lds = xb > sb ? xb : sb;
+    // x goes through LDS above 16 rows (64x5120x1280 14.7 -> 7.9 us, 64x1280x5120 22 -> 11.6), in wide layers above 8 (51865x1280
+    // for 16 14.1 us, direct 16.7; for 4 9.0 and 8.7).  At 16 rows of a layer that is not wide it is a matter of K: 16x5120x1280
+    // 5.5 us, direct 6.0, but 16x1280x5120 10.1 and 8.5.
+    if (a.M > (wide ? 8 : 16)) {
+        // rows of x a workgroup takes: 16, or 32 where the weights are too many to come from a cache the second time
+        // (64x51865x1280 29 us, 16 rows 36, 64 rows 32); fp32 has no registers for them (48x20000x2048 29 us, 43)
+        const int mt = P == 1 && wide && a.M > 16 ? 2 : 1, rb = (a.M + 16 * mt - 1) / (16 * mt);
+        const int nt = (long)(a.tiles + PAIR - 1) / PAIR * rb < W4_GROUPS ? 1 : PAIR;
+        const int groups = (a.tiles + nt - 1) / nt, rows = a.M < 16 * mt ? a.M : 16 * mt;
+        a.kw = 1;                                                // ways that share the chunks: as few as fill the chip
+        while (a.kw < W4_WAVES && a.kw < a.chunks && (long)groups * rb * a.kw < W4_WAVES * W4_GROUPS) a.kw *= 2;
         const int tw = W4_WAVES / a.kw;
-        const dim3 grid((groups + tw - 1) / tw, (a.M + 16 * mt - 1) / (16 * mt)), block(64 * W4_WAVES);
-#define L(MT, NT) hipLaunchKernelGGL((w4_staged_kernel<TX, GS, MT, NT>), grid, block, lds, s, a)
-        if (mt == 1) L(1, pair); else if (mt == 2) L(2, 1); else L(4, 1);
+        const dim3 grid((groups + tw - 1) / tw, rb), block(64 * W4_WAVES);
+        const int room = (long)grid.x * rb <= 256 ? 2 * W4_X_BYTES : W4_X_BYTES, most = (room / (rows * P) - 16) / 256;
+        const int blocks = (a.chunks + most - 1) / most;
+        a.block = (a.chunks + blocks - 1) / blocks;              // blocks of one size, and whole rounds of the ways
+        if (blocks > 1 && most >= a.kw) {
+            a.block = (a.block + a.kw - 1) / a.kw * a.kw;
+            if (a.block > most) a.block = most / a.kw * a.kw;
+        }
+        const int xb = rows * P * (a.block * 256 + 16), sb = a.kw > 1 ? W4_WAVES * nt * mt * 1024 : 0, lds = xb > sb ? xb : sb;
+#define L(MT, NT)                                                                                                        \
+    do {                                                                                                                 \
+        static avsr_dev_flags set;                                                                                       \
+        if (lds > 65536 && !avsr_allow_lds((const void*)w4_staged_kernel<TX, GS, MT, NT>, 2 * W4_X_BYTES, set)) return AVSR_EHIP; \
+        hipLaunchKernelGGL((w4_staged_kernel<TX, GS, MT, NT>), grid, block, lds, s, a);                                  \
+    } while (0)
+        if (mt == 2) L(PAIR, PAIR);
+        else if (nt == 2) L(1, PAIR);
+        else L(1, 1);
 #undef L
         return avsr_launch_status();
     }
-    const int nt = wide ? 2 : 1, groups = (a.tiles + nt - 1) / nt, mt_d = P == 3 && mt == 4 ? 2 : mt;      // fp32: three times the registers
+    const int nt = wide ? 2 : 1, groups = (a.tiles + nt - 1) / nt;
     int waves = W4_FILL / groups;                                // no more than there are chunks
     waves = waves < 1 ? 1 : waves > W4_WAVES ? W4_WAVES : waves;
     waves = waves < a.chunks ? waves : a.chunks;
-    const dim3 grid(groups, (a.M + 16 * mt_d - 1) / (16 * mt_d)), block(64 * waves);
-    const int lds = waves > 1 ? waves * nt * mt_d * 1024 : 0;
-#define L(MT, NT) hipLaunchKernelGGL((w4_direct_kernel<TX, GS, MT, NT, (P * MT * NT <= 3)>), grid, block, lds, s, a)
-    if (nt == 2) L(1, 2);
-    else if (mt_d == 1) L(1, 1);
-    else if (mt_d == 2) L(2, 1);
-    else if constexpr (P == 1) L(4, 1);
-#undef L
+    const dim3 grid(groups), block(64 * waves);
+    const int lds = waves > 1 ? waves * nt * 1024 : 0;
+    if (nt == 2) hipLaunchKernelGGL((w4_direct_kernel<TX, GS, 2, P == 1>), grid, block, lds, s, a);
+    else hipLaunchKernelGGL((w4_direct_kernel<TX, GS, 1, true>), grid, block, lds, s, a);
     return avsr_launch_status();
 }
 
@@ -340,7 +360,7 @@ extern "C" int avsr_w4_matmul(avsr_stream_t stream, int x_dtype, int out_dtype, 
     if ((x_dtype != AVSR_F32 && x_dtype != AVSR_BF16) || (out_dtype != AVSR_F32 && out_dtype != AVSR_BF16)) return AVSR_EINVAL;
     if (act != AVSR_ACT_NONE && act != AVSR_ACT_GELU && act != AVSR_ACT_RELU) return AVSR_EINVAL;
     if (group != 32 && group != 64 && group != 128) return AVSR_EUNSUPPORTED;
-    if (((uintptr_t)packed % 16) || ((uintptr_t)scales % 8) || N > (1LL << 28) || K > (1LL << 24) || M > (1 << 20)) return AVSR_EUNSUPPORTED;
+    if (((uintptr_t)packed % 16) || ((uintptr_t)scales % 8) || N > (1LL << 28) || K > (1LL << 24) || M > (1 << 19)) return AVSR_EUNSUPPORTED;
     if (M == 0) return AVSR_OK;
     const int xs = x_dtype == AVSR_F32 ? 4 : 8;
     const bool of = out_dtype == AVSR_F32;

@@ -423,7 +423,11 @@ def w4_check(dev, M, N, K, group, xt, ot, *, act=ops.ACT_NONE, bias=True, residu
     assert (err <= worst + HALF[ot] * (y.abs() + worst) + 1e-30).all()
     # and as a whole: the roundings are independent, about sqrt(K / 32) of them on sums of up to 24 sqrt(group) |x| scale,
     # against |y| = 4.6 sqrt(K) |x| scale: below 40 half steps; the result's own rounding is uniform, HALF / sqrt(3)
-    assert err.norm() <= (40 * U32 + HALF[ot] * 0.6 + 1e-7) * y.norm()
+    # - of many values.  Fewer than 16 different ones are no average: n copies of one value y have n times one error of up to
+    # HALF |y|, so that |err| / |y| <= HALF (20 rows of one column whose weight is 0 are 20 times the bias: 1.2456 is 2.73e-3 of
+    # itself away from the next bf16, HALF 3.91e-3).
+    one = 0.6 if y.unique().numel() >= 16 else 1.0
+    assert err.norm() <= (40 * U32 + HALF[ot] * one + 1e-7) * y.norm()
 
 
 @pytest.mark.parametrize("xt,ot", [(BF, BF), (BF, F32), (F32, F32), (F32, BF)])
@@ -445,6 +449,16 @@ def test_w4_wide(dev, xt, M, N, K):
 @pytest.mark.parametrize("M,N,K,pad", [(3, 16400, 200, 0), (5, 16385, 1000, 0), (16, 16400, 333, 5), (4, 16384, 4480, 0), (33, 16390, 1160, 0), (70, 16384, 130, 0)])
 def test_w4_wide_through_lds(dev, xt, ot, group, M, N, K, pad):
     """Wide layers: x in one block and in several, rows that are not aligned, more rows than a workgroup takes."""
+    w4_check(dev, M, N, K, group, xt, ot, pad=pad, residual=bool(pad), act=ops.ACT_GELU if pad else ops.ACT_NONE)
+
+
+@pytest.mark.parametrize("xt,ot", [(BF, BF), (F32, F32)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K,pad", [(17, 1280, 4500, 0), (40, 640, 9000, 0), (33, 300, 2333, 5), (64, 5120, 300, 0), (100, 4000, 1290, 0), (200, 2600, 130, 3),
+                                       (18, 40, 16500, 0), (40, 16400, 2200, 0), (20, 1, 1, 0)])
+def test_w4_layers_through_lds(dev, xt, ot, group, M, N, K, pad):
+    """More than 16 rows: one way to eight that share the columns, one block of x and several, more columns than a block, fewer
+    than a chunk, last tiles and rows that are not whole."""
     w4_check(dev, M, N, K, group, xt, ot, pad=pad, residual=bool(pad), act=ops.ACT_GELU if pad else ops.ACT_NONE)
 
 
