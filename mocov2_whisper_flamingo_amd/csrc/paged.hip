@@ -905,6 +905,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
 }
+// The compiler puts no wait between a matrix instruction and inline assembly that reads its result: scores pass through here
+// before the maximum is taken of them straight away (12 wait states, what the compiler leaves before an instruction of its own).
+__device__ __forceinline__ void settle(f32x16& a, f32x16& b) { asm volatile("s_nop 11" : "+v"(a), "+v"(b)); }
 __device__ __forceinline__ float max16(const f32x16& s) {
     float a = max3(s[0], s[1], s[2]), b = max3(s[3], s[4], s[5]);
     a = max3(a, s[6], s[7]); b = max3(b, s[8], s[9]);
@@ -1095,6 +1098,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
         f32x16 s[2];
         scores(K, s[0]);
         scores(K + 64 * D, s[1]);
+        settle(s[0], s[1]);
         const float mx = fmaxf(max16(s[0]), max16(s[1]));
         if (__any(mx > thr)) move_reference(mx);
 #pragma unroll

@@ -245,6 +245,26 @@ def test_attn_into_its_own_queries(dev, dtype, lens, news):
 
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,news", [([300, 200, 64, 3], [130, 70, 1, 3]), ([4000] * 6, [200] * 6), ([2000] * 80, [1] * 80), ([9000, 30], [2, 1])])
+def test_attn_repeats_bit_for_bit(dev, dtype, D, lens, news):
+    """Nothing in a call depends on timing: no order of atomics, no score read before its matrix instruction is done."""
+    g = torch.Generator(device=dev).manual_seed(10)
+    start = [0]
+    for n in news:
+        start.append(start[-1] + n)
+    W = up(max(lens), 64)
+    kv = torch.randn(len(lens) * W, 2, 2, 64, D, generator=g, device=dev).to(dtype)
+    table = torch.arange(len(lens) * W, dtype=torch.int32, device=dev).view(-1, W)
+    q = 4 * torch.randn(start[-1], 4, D, generator=g, device=dev).to(dtype)
+    call = lambda: ops.paged_attn(q, kv[:, 0], kv[:, 1], table, i32(lens, dev), i32(start, dev), scale=D ** -0.5)
+    want = call()
+    assert torch.isfinite(want.float()).all()
+    for _ in range(20):
+        assert torch.equal(call(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("news", [[3, 2], [70, 90], [200, 40]])
 @pytest.mark.parametrize("G", [1, 3])
 def test_attn_values_that_are_not_finite_inside_a_chunk(dev, dtype, D, news, G):
