@@ -326,7 +326,7 @@ extern "C" int avsr_paged_write(avsr_stream_t stream, int in_dtype, int page_dty
     const int64_t n = rows * 2 * H * head_dim / ((in_dtype == AVSR_F32 && page_dtype == AVSR_F32) ? 4 : 8);
     hipStream_t s = (hipStream_t)stream;
     const int64_t blocks = (n + 1023) / 1024;
-    if (blocks > 0x7fffffff) return AVSR_EUNSUPPORTED;
+    if (blocks > 0xffffff) return AVSR_EUNSUPPORTED;             // a launch has fewer than 2^32 threads
 #define L(TI, TO) hipLaunchKernelGGL((paged_write_kernel<TI, TO, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a)
     if (in_dtype == AVSR_BF16 && page_dtype == AVSR_BF16) L(bf16_t, bf16_t);
     else if (in_dtype == AVSR_F32 && page_dtype == AVSR_F32) L(float, float);
@@ -352,7 +352,8 @@ struct AttnArgs {
     const int* lens; const int* q_start;
     void* o; long ldo, ho;
     int B, Hk, G, N, shift, n_pages; float c; int causal;     // c = scale * log2(e)
-    int splits, few_rows;                         // key splits; largest request of the first kernel (0 = any)
+    int splits, few_rows;                         // key splits; most rows of a request that the first kernel takes (0 = any)
+    int n_few, few_tiles;                         // second kernel: workgroups in its grid that do the first one's work, tiles of 16 rows
     float *part, *part_ml;                        // [rows][splits][D] sums and [rows][splits]{m, l} of a split grid
 };
 
@@ -696,14 +697,13 @@ template <int D> __device__ __forceinline__ void store_vals(float* p, const floa
 // 16 cost the matrix pipe nothing that the memory would not take longer for: 64 requests x 20 heads x 1500 keys (492 MB) in
 // 85 us, 5.8 TB/s, the rate of a long read; 4 requests of 7000 to 32700 keys, 8 heads of 128 (271 MB), 56 us and 5 for the
 // join; 8 requests x 6 heads x 440 keys 7 us, a launch and three dependent trips to memory.
+template <int D, int WAVES> struct FewLds { float m[WAVES][16], l[WAVES][16], o[WAVES][16][D + 4]; };
 template <typename T, int D, int WAVES, bool AHEAD>
-__global__ __launch_bounds__(64 * WAVES, D == 128 ? 2 : sizeof(T) == 4 || AHEAD ? 3 : 4) void paged_attn_few_kernel(AttnArgs a) {
+__device__ __forceinline__ void attn_few(const AttnArgs& a, FewLds<D, WAVES>& lds, int bx, int by, int ny) {
     typedef Frag<T, D> F;
-    __shared__ float s_m[WAVES][16], s_l[WAVES][16];
-    __shared__ float s_o[WAVES][16][D + 4];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x % a.splits, x = blockIdx.x / a.splits;
+    const int split = bx % a.splits, x = bx / a.splits;
     const int hk = x % a.Hk, b = x / a.Hk;
     const int* row = a.table + b * a.ld_table;
     Stage<F> sg[AHEAD ? 2 : 1];
@@ -716,7 +716,7 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 2 : sizeof(T) == 4 || AHEAD 
     const Req r = request(a, b);
     const int rows = r.nq * a.G;
     if (a.few_rows && rows > a.few_rows) return;
-    for (int r0 = blockIdx.y * 16; r0 < rows; r0 += gridDim.y * 16) {
+    for (int r0 = by * 16; r0 < rows; r0 += ny * 16) {
         const int n_rows = min(16, rows - r0);
         const int tok0 = r0 / a.G, tok1 = (r0 + n_rows - 1) / a.G;
         const int base = a.causal ? r.len - r.nq : r.len - 1;               // last key of token t: base + t (causal) or base
@@ -732,30 +732,30 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 2 : sizeof(T) == 4 || AHEAD 
         attend<F, T, 1, D, AHEAD>(st, a, q, limit, row, hk, t0 + w, WAVES, t1, kmin, kmax, lane, sg, loaded);
         loaded = false;
         st.l[0] = xor_add<32>(xor_add<16>(st.l[0]));
-        if (g == 0) { s_m[w][i] = st.m[0]; s_l[w][i] = st.l[0]; }
+        if (g == 0) { lds.m[w][i] = st.m[0]; lds.l[w][i] = st.l[0]; }
         if (i < n_rows) {
 #pragma unroll
             for (int rr = 0; rr < 4; ++rr)
 #pragma unroll
-                for (int e = 0; e < D / 16; ++e) s_o[w][i][(D / 4) * g + (D / 16) * rr + e] = st.o[0][e][rr];
+                for (int e = 0; e < D / 16; ++e) lds.o[w][i][(D / 4) * g + (D / 16) * rr + e] = st.o[0][e][rr];
         }
         __syncthreads();
         // 8 columns a thread
         for (int c = threadIdx.x; c < n_rows * (D / 8); c += 64 * WAVES) {
             const int rw = c / (D / 8), d = (c % (D / 8)) * 8;
-            float m = s_m[0][rw];
+            float m = lds.m[0][rw];
 #pragma unroll
-            for (int u = 1; u < WAVES; ++u) m = fmaxf(m, s_m[u][rw]);
+            for (int u = 1; u < WAVES; ++u) m = fmaxf(m, lds.m[u][rw]);
             const float ref = m == -INFINITY ? 0.f : m;
             float l = 0.f, o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) o[j] = 0.f;
 #pragma unroll
             for (int u = 0; u < WAVES; ++u) {
-                const float f = __builtin_amdgcn_exp2f(s_m[u][rw] - ref);
-                l = fmaf(f, s_l[u][rw], l);
+                const float f = __builtin_amdgcn_exp2f(lds.m[u][rw] - ref);
+                l = fmaf(f, lds.l[u][rw], l);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = fmaf(f, s_o[u][rw][d + j], o[j]);
+                for (int j = 0; j < 8; ++j) o[j] = fmaf(f, lds.o[u][rw][d + j], o[j]);
             }
             const int t = (r0 + rw) / a.G, h = hk * a.G + (r0 + rw) - t * a.G;
             if (a.splits == 1) {
@@ -771,6 +771,11 @@ __global__ __launch_bounds__(64 * WAVES, D == 128 ? 2 : sizeof(T) == 4 || AHEAD 
         }
         __syncthreads();
     }
+}
+template <typename T, int D, int WAVES, bool AHEAD>
+__global__ __launch_bounds__(64 * WAVES, D == 128 ? 2 : sizeof(T) == 4 || AHEAD ? 3 : 4) void paged_attn_few_kernel(AttnArgs a) {
+    __shared__ FewLds<D, WAVES> lds;
+    attn_few<T, D, WAVES, AHEAD>(a, lds, blockIdx.x, blockIdx.y, gridDim.y);
 }
 
 // Joins the splits of a row, a wave per row: lane s weighs split s, then every lane adds up its columns.
@@ -899,7 +904,11 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnArgs a) {
 // has a maximum, a multiply-add, an exponential, an addition and half a conversion to do, more cycles than the matrix pipe
 // needs for the two products of a 64-column head: the maximum is only compared (the reference point moves when a score
 // exceeds it by 2^8), the scale's sign is taken into Q so that raw scores can be compared.  16 requests of 512 tokens on
-// 4096 keys, 16 heads over 4: 171 us (754 TF) with 64 columns, 152 us (848 TF) with 8 heads of 128; 64 rows a wave 184 us.
+// 4096 keys, 16 heads over 4: 168 us (768 TF) with 64 columns, 145 us (890 TF) with 8 heads of 128; 64 rows a wave 184 us.
+// Requests with few rows, bound by memory, are in the same grid: beside the matrix products of the others (64 requests of 1 to 512
+// tokens on 1000 to 4000 keys, 16 heads over 4: 65 us, as two launches 100; 32 of 1 to 1000 on up to 6000, 32 heads of 128 over
+// 8: 173, 226).  They start behind as many of the large ones as fill half the chip's places, which then lie evenly on the CUs: in
+// front of all of them 64 requests of 1 to 224 tokens take 37 us, behind them 29 but the batch of 32 227, here 29 and 173.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -965,10 +974,21 @@ template <int D>
 __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(AttnArgs a) {
     typedef KvTile<D> L;
     typedef bf16_t T;
-    __shared__ __attribute__((aligned(16))) bf16_t Ks[2][64 * D], Vs[2][64 * D];
+    __shared__ union { struct { bf16_t k[2][64 * D], v[2][64 * D]; } kv; FewLds<D, 4> few; } lds __attribute__((aligned(16)));
+    auto &Ks = lds.kv.k, &Vs = lds.kv.v;
+    // The grid is runs of eight workgroups, one for each XCD, so that those of a kv head stay on theirs; the runs of requests with
+    // few rows stand behind the first FIRST of the others.
+    constexpr unsigned FIRST = D == 64 ? 64 : 32;
+    const unsigned run = blockIdx.x >> 3, few_runs = (unsigned)(a.n_few + 7) >> 3, first_runs = min((gridDim.x >> 3) - few_runs, FIRST);
+    if (run >= first_runs && run < first_runs + few_runs) {
+        const int ny = a.few_tiles, nx = a.n_few / ny, at = (int)(blockIdx.x - 8 * first_runs);
+        if (at < a.n_few) attn_few<T, D, 4, false>(a, lds.few, at % nx, at / nx, ny);
+        return;
+    }
+    const int id = (int)(run < first_runs ? blockIdx.x : blockIdx.x - 8 * few_runs);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int r32 = lane & 31, hf = lane >> 5;
-    const int hk = blockIdx.x % a.Hk, split = blockIdx.x / a.Hk % a.splits, tile = blockIdx.x / a.Hk / a.splits;
+    const int hk = id % a.Hk, split = id / a.Hk % a.splits, tile = id / a.Hk / a.splits;
     const RowTile rt = row_tile<128>(a, tile, lane);
     const Req r = rt.r;
     if (rt.rows <= a.few_rows || rt.r0 < 0 || rt.r0 >= rt.rows) return;
@@ -1229,14 +1249,17 @@ template <typename T, int D>
 static int launch_attn(hipStream_t s, AttnArgs a, const AttnPlan& p) {
     const dim3 few((unsigned)p.grid_few, p.tiles_few);
     constexpr bool small = sizeof(T) * D <= 128;
+    if constexpr (sizeof(T) == 2) {
+        if (p.chunk) hipLaunchKernelGGL((paged_attn_chunk_kernel<D>), dim3((unsigned)((p.grid_chunk + 7) / 8 + (a.n_few + 7) / 8) * 8), dim3(256), 0, s, a);
+    }
+    const bool first = p.few && !(sizeof(T) == 2 && p.chunk);
 #define L(WAVES, AHEAD) hipLaunchKernelGGL((paged_attn_few_kernel<T, D, WAVES, AHEAD>), few, dim3(64 * WAVES), 0, s, a)
-    if (p.few && p.waves == 8) L(8, small);
-    else if (p.few && small && p.ahead) L(4, small);
-    else if (p.few) L(4, false);
+    if (first && p.waves == 8) L(8, small);
+    else if (first && small && p.ahead) L(4, small);
+    else if (first) L(4, false);
 #undef L
-    if (p.chunk) {
-        if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((paged_attn_rows_kernel<T, D, D == 64 ? 2 : 1>), dim3((unsigned)p.grid_chunk), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((paged_attn_chunk_kernel<D>), dim3((unsigned)p.grid_chunk), dim3(256), 0, s, a);
+    if constexpr (sizeof(T) == 4) {
+        if (p.chunk) hipLaunchKernelGGL((paged_attn_rows_kernel<T, D, D == 64 ? 2 : 1>), dim3((unsigned)p.grid_chunk), dim3(256), 0, s, a);
     }
     if (p.splits > 1) hipLaunchKernelGGL((paged_attn_join_kernel<T, D>), dim3((unsigned)(((int64_t)a.N * a.Hk * a.G + 3) / 4)), dim3(256), 0, s, a);
     return avsr_launch_status();
@@ -1266,11 +1289,13 @@ extern "C" int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, i
     const int64_t mq = max_q < N ? max_q : N, mk = max_k < width * page ? max_k : width * page;
     const AttnPlan p = attn_plan(dtype, head_dim, N, B, Hk, Hq / Hk, mq, mk);
     if (p.floats && (!workspace || workspace_bytes < p.floats * 4 || (uintptr_t)workspace % 16)) return AVSR_EINVAL;
-    if (p.grid_few > 0x7fffffff || p.grid_chunk > 0x7ffffff0) return AVSR_EUNSUPPORTED;
+    const int64_t n_few = p.chunk ? p.grid_few * p.tiles_few : 0;
+    // a launch has fewer than 2^32 threads
+    if (p.grid_few > 0xffffff || p.grid_chunk + n_few > 0xfffff0 || (p.splits > 1 && N * Hq > 0x3ffffff)) return AVSR_EUNSUPPORTED;
     float* part = (float*)workspace;
     AttnArgs a = {q, ldq, q_head, k_pages, v_pages, k_page_stride, k_head_stride, v_page_stride, v_head_stride, table, ld_table, (int)width,
                   lens, q_start, o, ldo, o_head, (int)B, (int)Hk, (int)(Hq / Hk), (int)N, shift, (int)n_pages, scale * LOG2E, causal != 0,
-                  p.splits, p.few_rows, part, part ? part + N * Hq * p.splits * head_dim : nullptr};
+                  p.splits, p.few_rows, (int)n_few, p.tiles_few, part, part ? part + N * Hq * p.splits * head_dim : nullptr};
     hipStream_t s = (hipStream_t)stream;
     if (dtype == AVSR_BF16) return head_dim == 64 ? launch_attn<bf16_t, 64>(s, a, p) : launch_attn<bf16_t, 128>(s, a, p);
     return head_dim == 64 ? launch_attn<float, 64>(s, a, p) : launch_attn<float, 128>(s, a, p);
