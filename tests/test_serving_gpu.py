@@ -558,6 +558,43 @@ def test_embed_tokens_at(dev):
         assert flag.item() == 1
 
 
+def test_calls_on_two_streams_at_once(dev):
+    """Split attention, a mixed batch, products and a plan on two streams, each with operands of its own: what one stream alone gives."""
+    g = torch.Generator(device=dev).manual_seed(12)
+
+    def work(k):
+        lens, news = [(9000, 700, 40), (5000, 64, 333)][k], [(1, 130, 3), (2, 1, 70)][k]
+        W = up(max(lens), 64)
+        kv = torch.randn(3 * W, 2, 2, 64, 64, generator=g, device=dev).to(BF)
+        table = torch.arange(3 * W, dtype=torch.int32, device=dev).view(3, W)
+        q = torch.randn(sum(news), 4, 64, generator=g, device=dev).to(BF)
+        w = ops.w4_quantize(torch.randn(1000, 2200, generator=g, device=dev))
+        x = torch.randn(24, 2200, generator=g, device=dev)
+        state = (i32(list(lens), dev), i32(list(news), dev), i32([0, news[0], news[0] + news[1], sum(news)], dev))
+        ring, pool = torch.arange(3 * W, dtype=torch.int32, device=dev), i32([0, 3 * W], dev)
+
+        def call():
+            lo, po = torch.empty_like(state[0]), torch.empty_like(pool)
+            plan = ops.paged_plan(torch.zeros_like(state[0]), state[1], table.clone(), ring.clone(), pool, 64, 300, lens_out=lo, pool_out=po)
+            return (ops.paged_attn(q, kv[:, 0], kv[:, 1], table, state[0], state[2], scale=0.125),
+                    ops.paged_attn(q[:1], kv[:, 0], kv[:, 1], table[:1], state[0][:1], i32([0, 1], dev), max_q=1, scale=0.125),
+                    ops.w4_matmul(x, w), ops.w4_matmul(x[:3], w), plan.slots, plan.q_start, lo, po)
+        return call
+
+    calls = [work(0), work(1)]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                got.append(c())
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
 def test_serving_step_captured_and_replayed(dev):
     """Plan, write and attention of a step in a graph: every replay moves the cache on by a token, as eager calls do."""
     g = torch.Generator().manual_seed(12)
