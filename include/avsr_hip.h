@@ -546,6 +546,8 @@ int avsr_adamw_step_dev(avsr_stream_t stream, float* param, float* grad, float* 
  * Serving the Whisper decoder (hf modeling_whisper.py:649-797 with past_key_values) to requests of different lengths
  * that come and go.  The keys and values of `page` tokens of one layer form a page: element (p, h, t, d) at
  * pages + p*page_stride + h*head_stride + t*head_dim + d.  page: 16, 32, 64, 128 or 256; head_dim: 64 or 128.
+ * Tensors and their strides are multiples of 16 bytes (the stride of a dimension of one counts for nothing); rows times heads
+ * stay within 2^30, pages times `page` and the tokens of a request too.
  * A request holds its pages in a row of a block table (int32, ld_table >= width), token j in entry j / page.
  *
  * avsr_paged_plan: the tables of one step, from the requests' lengths, on the GPU.  add[b] >= 0: request b adds that
@@ -594,9 +596,9 @@ int avsr_embed_tokens_at(avsr_stream_t stream, int table_dtype, const int64_t* i
  * decoder's nn.Linear layers (hf:277-281,374-376) on 4-bit weights.  packed: 32-bit words of eight nibbles,
  * word[n/16][k/128][k/8 % 4][n % 16][k/32 % 4], the nibble of k % 8 = e at bit 4*(e/2) + 16*(e%2); scales: bf16
  * [n/16][k/group][n % 16]; both padded to whole tiles of 16 rows and 128 columns with nibble 8 and scale 0.
- * group: 32, 64 or 128.  x fp32 or bf16, y and residual fp32 or bf16 (residual of y's type, may be y itself); act NONE,
- * GELU or RELU.  fp32 sums, which pass through some thousand times the largest x: it is at most 1e34 in magnitude.  A row
- * of x with a value that is not finite yields NaN. */
+ * group: 32, 64 or 128; M up to 2^19, N to 2^28, K to 2^24.  x fp32 or bf16, y and residual fp32 or bf16 (residual of y's
+ * type, may be y itself); act NONE, GELU or RELU.  fp32 sums, which pass through some thousand times the largest x: it is at
+ * most 1e34 in magnitude.  A row of x with a value that is not finite yields NaN. */
 int avsr_w4_matmul(avsr_stream_t stream, int x_dtype, int out_dtype, const void* x, int64_t ldx, const void* packed,
                    const void* scales, int64_t group, const float* bias, int act, const void* residual, int64_t ldr,
                    void* y, int64_t ldy, int64_t M, int64_t N, int64_t K);

@@ -1089,7 +1089,7 @@ def paged_plan(lens, new, table, ring, pool, page_size, max_tokens, *, lens_out=
 
 
 def paged_write(k, v, k_pages, v_pages, slots):
-    """k, v [N, H, D] (rows and heads of any stride) into the pages [pages, H, page, D] at ``slots`` int32 [N] =
+    """k, v [N, H, D] (rows and heads at any multiple of 16 bytes) into the pages [pages, H, page, D] at ``slots`` int32 [N] =
     page * page_size + place (``PagedPlan.slots``); a row with a negative slot is left out, the others are distinct.  fp32 rows are
     rounded into bf16 pages."""
     n, H, page, D, kp, kh, vp, vh = _pages(k_pages, v_pages)
