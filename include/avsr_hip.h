@@ -576,8 +576,8 @@ int avsr_paged_write(avsr_stream_t stream, int in_dtype, int page_dtype, const v
  * of request b, which holds lens[b] tokens with them (avsr_paged_plan's lens_out): row i of n sees the keys up to
  * lens[b] - n + i (causal) or all lens[b] of them.  Query head h reads kv head h / (Hq / Hk).  A row that sees no key
  * yields zeros; rows behind q_start[B] are left as they were; a key that a row does not see has no influence on it,
- * whatever it holds; a table entry that names no page hides its keys.  Softmax statistics and sums in fp32; bf16 rounds
- * the probabilities to bf16 for the second product.  max_q, max_k: at most so many new tokens and keys in any request;
+ * whatever it holds; a table entry that names no page hides its keys.  Softmax statistics and sums in fp32; with
+ * bf16 the probabilities enter the second product as two bf16 values each (2^-16 of themselves).  max_q, max_k: at most so many new tokens and keys in any request;
  * they choose the grid, larger requests still come out right.  o may be q.  Results do not depend on the workspace's contents. */
 int64_t avsr_paged_attn_workspace_bytes(int dtype, int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim,
                                         int64_t max_q, int64_t max_k);

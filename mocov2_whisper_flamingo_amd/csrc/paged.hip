@@ -376,6 +376,21 @@ __device__ __forceinline__ unsigned finite_half(unsigned v, bool& odd) {
     return v & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
 }
 
+// Probabilities go into the second product as the sum of two bf16 values, the nearest one and the nearest to what is left: off by
+// 2^-16 of themselves at most, so that a bf16 result is the exact one rounded once but for values next to a border (one value alone: 2^-8;
+// against 64 bits 2.2e-3 of the result's norm where its own rounding is 1.66e-3).  The rest comes of one instruction, x - (hi . {1, 0}),
+// exact because its bits are x's own.
+struct Two { bf16x2 hi, lo; };
+__device__ __forceinline__ Two two_pieces(float x, float y) {
+    unsigned first = 0x0000BF80u, second = 0xBF800000u;               // {-1, 0} and {0, -1}; opaque: as an inline constant -1.0 has two meanings
+    asm("" : "+s"(first), "+s"(second));
+    Two t;
+    t.hi = (bf16x2){(bf16_t)x, (bf16_t)y};
+    t.lo = (bf16x2){(bf16_t)__builtin_amdgcn_fdot2_f32_bf16(t.hi, __builtin_bit_cast(bf16x2, first), x, false),
+                    (bf16_t)__builtin_amdgcn_fdot2_f32_bf16(t.hi, __builtin_bit_cast(bf16x2, second), y, false)};
+    return t;
+}
+
 template <typename T, int D> struct Frag;
 // ---- bf16: v_mfma_f32_16x16x32_bf16 (A row / B column lane & 15, k = 8g + j; C column lane & 15, row 4g + r)
 template <int D> struct Frag<bf16_t, D> {
@@ -425,12 +440,17 @@ template <int D> struct Frag<bf16_t, D> {
             f[p] = __builtin_amdgcn_perm(v.x[2 * p + 1][e >> 1], v.x[2 * p][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
         return __builtin_bit_cast(bf16x8, f);
     }
-    // P rounds to bf16 for the product (half a step of 2^-8 relative each, averaged over the keys; the row sum stays fp32)
-    static __device__ __forceinline__ bf16x8 probs(const f32x4 (&p)[2]) {
-        bf16x8 b;
+    static constexpr bool TWO = true;                                    // probabilities are two pieces
+    struct P { bf16x8 hi, lo; };
+    static __device__ __forceinline__ P probs(const f32x4 (&s)[2]) {
+        P p;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) { b[r] = (bf16_t)p[0][r]; b[4 + r] = (bf16_t)p[1][r]; }
-        return b;
+        for (int r = 0; r < 8; r += 2) {
+            const Two t = two_pieces(s[r >> 2][r & 3], s[r >> 2][(r & 3) + 1]);
+            p.hi[r] = t.hi[0]; p.hi[r + 1] = t.hi[1];
+            p.lo[r] = t.lo[0]; p.lo[r + 1] = t.lo[1];
+        }
+        return p;
     }
     static __device__ __forceinline__ void zero_key(V& v, int j) { v.x[j] = (vrow_t)(0u); }
     static __device__ __forceinline__ int key_of_v(int j, int g) { return 8 * g + j; }
@@ -442,8 +462,9 @@ template <int D> struct Frag<bf16_t, D> {
             for (int w = 0; w < VW / 2; ++w) v.x[j][w] = finite_half(v.x[j][w], odd);
         return odd;
     }
-    static __device__ __forceinline__ f32x4 pv(const V& v, int e, const f32x4 (&p)[2], f32x4 o) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(column(v, e), probs(p), o, 0, 0, 0);
+    static __device__ __forceinline__ f32x4 pv(const V& v, int e, const P& p, f32x4 o) {
+        const bf16x8 c = column(v, e);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, p.hi, __builtin_amdgcn_mfma_f32_16x16x32_bf16(c, p.lo, o, 0, 0, 0), 0, 0, 0);
     }
 };
 // ---- fp32: v_mfma_f32_16x16x4_f32 (A row / B column lane & 15, k = g; C as above)
@@ -508,9 +529,12 @@ template <int D> struct Frag<float, D> {
                 }
         return odd;
     }
-    static __device__ __forceinline__ f32x4 pv(const V& v, int e, const f32x4 (&p)[2], f32x4 o) {
+    static constexpr bool TWO = false;
+    struct P { f32x4 x[2]; };
+    static __device__ __forceinline__ P probs(const f32x4 (&s)[2]) { return {s[0], s[1]}; }
+    static __device__ __forceinline__ f32x4 pv(const V& v, int e, const P& p, f32x4 o) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x[j][e >> 2][e & 3], p[j >> 2][j & 3], o, 0, 0, 0);
+        for (int j = 0; j < 8; ++j) o = __builtin_amdgcn_mfma_f32_16x16x4f32(v.x[j][e >> 2][e & 3], p.x[j >> 2][j & 3], o, 0, 0, 0);
         return o;
     }
 };
@@ -617,8 +641,9 @@ __device__ __forceinline__ void attend_tile(State<NT, D>& st, const typename F::
                 sum += s[t][r];
             }
         st.l[n] += sum;
+        const typename F::P p = F::probs(s);
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) st.o[n][e] = F::pv(v, e, s, st.o[n][e]);
+        for (int e = 0; e < D / 16; ++e) st.o[n][e] = F::pv(v, e, p, st.o[n][e]);
     }
     if (odd) {
 #pragma unroll 1
@@ -640,7 +665,8 @@ __device__ __forceinline__ void attend_tile(State<NT, D>& st, const typename F::
 
 // Tiles first, first + step, ... < end of the request's keys.  AHEAD: the next tile's keys and values are in flight while a
 // tile is computed, its page numbers one tile further ahead; without, other waves' tiles are.  `loaded`: tile `first` is
-// already on its way.
+// already on its way.  An infinite value times a probability's second piece, which may be 0 or negative, is NaN where the first
+// piece alone gives an infinity: if that happens the tiles are gone through again as ones that a row sees in part.  Nothing else changes by it.
 template <typename F> struct Stage { typename F::K k; typename F::V v; TilePages tp; };
 template <typename F, typename T, int NT, int D, bool AHEAD>
 __device__ __forceinline__ void attend(State<NT, D>& st, const AttnArgs& a, const typename F::Q (&q)[NT], const int (&limit)[NT],
@@ -648,11 +674,7 @@ __device__ __forceinline__ void attend(State<NT, D>& st, const AttnArgs& a, cons
                                        Stage<F> (&sg)[AHEAD ? 2 : 1], bool loaded) {
     if (first >= end) return;
     const int i = lane & 15, g = lane >> 4;
-    if (!loaded) {
-        sg[0].tp = tile_pages(a, row, first);
-        load_tile<F, T>(a, sg[0].k, sg[0].v, sg[0].tp, first, hk, i, g, D);
-    }
-    TilePages next = tile_pages(a, row, first + step);
+    TilePages next;
     auto compute = [&](int kt, Stage<F>& s) {
         attend_tile<F, NT, D>(st, q, s.k, s.v, limit, hk, kt, kmin, kmax, s.tp, a, lane);
     };
@@ -661,20 +683,40 @@ __device__ __forceinline__ void attend(State<NT, D>& st, const AttnArgs& a, cons
         load_tile<F, T>(a, s.k, s.v, next, kt, hk, i, g, D);
         next = tile_pages(a, row, kt + step);
     };
-    if constexpr (AHEAD) {
-        for (int kt = first; kt < end; kt += 2 * step) {
-            if (kt + step < end) fetch(kt + step, sg[1]);
-            compute(kt, sg[0]);
-            if (kt + step < end) {
-                if (kt + 2 * step < end) fetch(kt + 2 * step, sg[0]);
-                compute(kt + step, sg[1]);
+    for (bool again = false;; again = true) {
+        if (!loaded) {
+            sg[0].tp = tile_pages(a, row, first);
+            load_tile<F, T>(a, sg[0].k, sg[0].v, sg[0].tp, first, hk, i, g, D);
+        }
+        next = tile_pages(a, row, first + step);
+        if constexpr (AHEAD) {
+            for (int kt = first; kt < end; kt += 2 * step) {
+                if (kt + step < end) fetch(kt + step, sg[1]);
+                compute(kt, sg[0]);
+                if (kt + step < end) {
+                    if (kt + 2 * step < end) fetch(kt + 2 * step, sg[0]);
+                    compute(kt + step, sg[1]);
+                }
+            }
+        } else {
+            for (int kt = first; kt < end; kt += step) {
+                compute(kt, sg[0]);
+                if (kt + step < end) fetch(kt + step, sg[0]);
             }
         }
-    } else {
-        for (int kt = first; kt < end; kt += step) {
-            compute(kt, sg[0]);
-            if (kt + step < end) fetch(kt + step, sg[0]);
+        bool nan = false;
+        if (F::TWO && !again) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) nan |= st.o[n][e][r] != st.o[n][e][r] && st.l[n] == st.l[n];
         }
+        if (!__any(nan)) return;
+        st.clear();
+        loaded = false;
+        kmin = -1;
     }
 }
 
@@ -901,10 +943,11 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnArgs a) {
 // bf16: tiles of 64 keys go to LDS once for the workgroup's four waves of 32 rows (LDS-DMA, two buffers, one barrier per
 // tile).  S^T and O^T as above on v_mfma_f32_32x32x16_bf16 (A row / B column lane & 31, k = 8 (lane / 32) + j; C column
 // lane & 31, row (i & 3) + 8 (i >> 2) + 4 (lane / 32)); V fragments come transposed out of LDS.  Per score the vector unit
-// has a maximum, a multiply-add, an exponential, an addition and half a conversion to do, more cycles than the matrix pipe
-// needs for the two products of a 64-column head: the maximum is only compared (the reference point moves when a score
+// has a maximum, a multiply-add, an exponential, an addition, a subtraction and a conversion to do, more cycles than the matrix
+// pipe needs for the products of a 64-column head: the maximum is only compared (the reference point moves when a score
 // exceeds it by 2^8), the scale's sign is taken into Q so that raw scores can be compared.  16 requests of 512 tokens on
-// 4096 keys, 16 heads over 4: 168 us (768 TF) with 64 columns, 145 us (890 TF) with 8 heads of 128; 64 rows a wave 184 us.
+// 4096 keys, 16 heads over 4: 241 us (535 TF) with 64 columns, 200 us (645 TF) with 8 heads of 128.  With probabilities of one bf16
+// value, two products of three, 169 and 148 us.
 // Requests with few rows, bound by memory, are in the same grid: beside the matrix products of the others (64 requests of 1 to 512
 // tokens on 1000 to 4000 keys, 16 heads over 4: 65 us, as two launches 100; 32 of 1 to 1000 on up to 6000, 32 heads of 128 over
 // 8: 173, 226).  They start behind as many of the large ones as fill half the chip's places, which then lie evenly on the CUs: in
@@ -929,21 +972,27 @@ template <int D> struct KvTile {
     // chunk c of a row stands at c ^ swizzle(row), so that neither fragment read below hits a bank twice
     static __device__ __forceinline__ int kswz(int row) { return D == 64 ? (row >> 1) & 7 : row & 15; }
     static __device__ __forceinline__ int vswz(int row) { return D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
-    // A fragment is read at a lane's offset (bytes, one per 16 or 32 columns, the same for every run of 32 keys) plus a constant.
-    // Keys: row lane & 31, columns 16 ks + 8 (lane / 32) ..
-    static __device__ __forceinline__ int koff(int ks, int lane) {
-        const int row = lane & 31;
-        return (row * D + (((2 * ks + (lane >> 5)) ^ kswz(row)) << 3)) * 2;
+    // A fragment is read at a lane's offset (bytes, the same for every run of 32 keys) plus a constant; the swizzle turns the column
+    // into an exclusive or of it.  It is made anew for every read: kept, the offsets would take registers that the accumulators need.
+    static __device__ __forceinline__ int flip(int off, int bits) {
+        asm("" : "+v"(off));
+        return off ^ bits;
     }
-    static __device__ __forceinline__ bf16x8 kfrag(const char* K, int off) { return *(const bf16x8*)(K + off); }
+    // Keys: row lane & 31, columns 16 ks + 8 (lane / 32) ..
+    static __device__ __forceinline__ int koff(int lane) {
+        const int row = lane & 31;
+        return (row * D + (((lane >> 5) ^ kswz(row)) << 3)) * 2;
+    }
+    static __device__ __forceinline__ bf16x8 kfrag(const char* K, int off, int ks) { return *(const bf16x8*)(K + (ks ? flip(off, 32 * ks) : off)); }
     // Values, transposed: columns 32 db + (lane & 31) of the keys 16 s2 + {0..3, 8..11} + 4 (lane / 32), the order of a score register's
     // keys.  16 lanes read four 32-byte pieces of four rows; which is a swizzle's bits do not depend on s2.
-    static __device__ __forceinline__ int voff(int db, int lane) {
-        const int i16 = lane & 15, row = 4 * (lane >> 5) + (i16 >> 2), col = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+    static __device__ __forceinline__ int voff(int lane) {
+        const int i16 = lane & 15, row = 4 * (lane >> 5) + (i16 >> 2), col = 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
         return (row * D + (((col >> 3) ^ vswz(row)) << 3) + (col & 7)) * 2;
     }
-    static __device__ __forceinline__ bf16x8 vfrag(const char* V, int s2, int off) {
+    static __device__ __forceinline__ bf16x8 vfrag(const char* V, int s2, int off, int db) {
         bf16x8 f;
+        if (db) off = flip(off, 64 * db);
 #pragma unroll
         for (int jh = 0; jh < 2; ++jh) {
             const char* p = V + off + (16 * s2 + 8 * jh) * D * 2;
@@ -976,6 +1025,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
     typedef bf16_t T;
     __shared__ union { struct { bf16_t k[2][64 * D], v[2][64 * D]; } kv; FewLds<D, 4> few; } lds __attribute__((aligned(16)));
     auto &Ks = lds.kv.k, &Vs = lds.kv.v;
+    __shared__ int again;
     // The grid is runs of eight workgroups, one for each XCD, so that those of a kv head stay on theirs; the runs of requests with
     // few rows stand behind the first FIRST of the others.
     constexpr unsigned FIRST = D == 64 ? 64 : 32;
@@ -1030,18 +1080,10 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
     // tile behind the DMA's back, and its wait would be one for the DMA
     int first = t0 * 64 >> a.shift;
     int entries = t0 < t1 ? row[min(first + lane, a.width - 1)] : 0;
-    unsigned kmove[L::PIECES], vmove[L::PIECES];
-#pragma unroll
-    for (int u = 0; u < L::PIECES; ++u) {
-        const int lr = (64 / L::CH) * u + lane / L::CH, ch = lane & (L::CH - 1), rw = 16 * w + lr;
-        kmove[u] = (lr * D + ((ch ^ L::kswz(rw)) << 3)) * 2;
-        vmove[u] = (lr * D + ((ch ^ L::vswz(rw)) << 3)) * 2;
-    }
-    int kr[D / 16], vr[D / 32];
-#pragma unroll
-    for (int ks = 0; ks < D / 16; ++ks) kr[ks] = L::koff(ks, lane);
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) vr[d] = L::voff(d, lane);
+    // where the lane's 16 bytes of a DMA piece (64 / CH rows, 1 KiB) come from; piece u of a run: 1024 u further, a key's chunk at ^ 4 u
+    const int lr = lane / L::CH, ch = lane & (L::CH - 1);
+    const unsigned kmove = (lr * D + ((ch ^ L::kswz(lr)) << 3)) * 2, vmove = (lr * D + ((ch ^ L::vswz(lr)) << 3)) * 2;
+    const int kr = L::koff(lane), vr = L::voff(lane);
     // Tile kt into a buffer; wave w moves run w of its four runs of 16 keys, of the keys and of the values.  Returns which of
     // the runs' pages exist.
     auto move = [&](int kt, int buf) {
@@ -1061,11 +1103,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
         const char* v = (const char*)((const T*)a.v + page * a.svp + hk * a.svh + in * D);
 #pragma unroll
         for (int u = 0; u < L::PIECES; ++u) {
-            dma_piece(k, kmove[u], (const char*)&Ks[buf][(16 * w) * D + u * 512]);
-            dma_piece(v, vmove[u], (const char*)&Vs[buf][(16 * w) * D + u * 512]);
+            dma_piece(k + 1024 * u, kmove ^ 64 * u, (const char*)&Ks[buf][(16 * w) * D + u * 512]);
+            dma_piece(v + 1024 * u, vmove, (const char*)&Vs[buf][(16 * w) * D + u * 512]);
         }
         return have;
     };
+    if (threadIdx.x == 0) again = 0;                             // set behind the barrier of the first tile at the earliest
     int kt = t0, buf = 0;
     unsigned next = t0 < t1 ? move(t0, 0) : 0;
     // Tile kt is in LDS for every wave, the next one on its way into the other buffer; which runs of this one have pages.
@@ -1091,8 +1134,8 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
 #pragma unroll
             for (int x = 0; x < 16; ++x) o[d][x] *= al;
     };
-    // Scores to probabilities: rounded to bf16 for the product (half a step of 2^-8 relative each); the sum is of the unrounded ones.
-    auto exponentials = [&](f32x16& s, bf16x8 (&p)[2]) {
+    // Scores to probabilities, in two pieces for the product; the sum is of the whole ones.
+    auto exponentials = [&](f32x16& s, bf16x8 (&hi)[2], bf16x8 (&lo)[2]) {
         float s0 = 0.f, s1 = 0.f;
 #pragma unroll
         for (int x = 0; x < 16; x += 2) {
@@ -1103,13 +1146,21 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
         }
         l += s0 + s1;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) { p[0][x] = (bf16_t)s[x]; p[1][x] = (bf16_t)s[8 + x]; }
+        for (int x = 0; x < 16; x += 2) {
+            const Two t = two_pieces(s[x], s[x + 1]);
+            hi[x >> 3][x & 7] = t.hi[0]; hi[x >> 3][(x & 7) + 1] = t.hi[1];
+            lo[x >> 3][x & 7] = t.lo[0]; lo[x >> 3][(x & 7) + 1] = t.lo[1];
+        }
+    };
+    auto product = [&](bf16x8 v, bf16x8 hi, bf16x8 lo, f32x16& o) {
+        o = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, lo, o, 0, 0, 0);
+        o = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, hi, o, 0, 0, 0);
     };
     auto scores = [&](const char* K, f32x16& s) {
 #pragma unroll
         for (int x = 0; x < 16; ++x) s[x] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(L::kfrag(K, kr[ks]), q[ks], s, 0, 0, 0);
+        for (int ks = 0; ks < D / 16; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(L::kfrag(K, kr, ks), q[ks], s, 0, 0, 0);
     };
     // A tile that every row sees whole, 64 keys at once: one look at the maximum, and the matrix pipe has the other half's
     // products to do while the vector unit makes the exponentials of one.
@@ -1123,13 +1174,12 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
         if (__any(mx > thr)) move_reference(mx);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-            bf16x8 p[2];
-            exponentials(s[st], p);
+            bf16x8 hi[2], lo[2];
+            exponentials(s[st], hi, lo);
 #pragma unroll
             for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
-                for (int d = 0; d < D / 32; ++d)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(L::vfrag(V + st * 64 * D, s2, vr[d]), p[s2], o[d], 0, 0, 0);
+                for (int d = 0; d < D / 32; ++d) product(L::vfrag(V + st * 64 * D, s2, vr, d), hi[s2], lo[s2], o[d]);
         }
     };
     // 32 keys of a tile that some row sees in part: values behind every row's last key are cleared, and ones that are not finite
@@ -1147,15 +1197,15 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
         }
         const float mx = max16(s);
         if (__any(mx > thr)) move_reference(mx);
-        bf16x8 p[2];
-        exponentials(s, p);
+        bf16x8 hi[2], lo[2];
+        exponentials(s, hi, lo);
         bool odd = false;
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
             for (int d = 0; d < D / 32; ++d) {
-                const u32x4 vf = cut_keys(__builtin_bit_cast(u32x4, L::vfrag(V, s2, vr[d])), k0 + 16 * s2, hf, (s2 ? ok1 : ok0) ? kmax : -1);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, finite_part(vf, odd)), p[s2], o[d], 0, 0, 0);
+                const u32x4 vf = cut_keys(__builtin_bit_cast(u32x4, L::vfrag(V, s2, vr, d)), k0 + 16 * s2, hf, (s2 ? ok1 : ok0) ? kmax : -1);
+                product(__builtin_bit_cast(bf16x8, finite_part(vf, odd)), hi[s2], lo[s2], o[d]);
             }
         if (__any(odd)) {
 #pragma unroll 1
@@ -1180,6 +1230,32 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
         have = arrive();
         if (have != 15u) break;
         whole_tile();
+    }
+    if (kt > t0) {
+        // An infinite value times a probability's second piece, which may be 0 or negative, is NaN where the first piece alone gives an
+        // infinity.  Every row sees these tiles whole: if it happened in one, the workgroup goes through them again by the second loop.
+        bool nan = false;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int x = 0; x < 16; ++x) nan |= o[d][x] != o[d][x] && l == l;
+        if (__any(nan)) again = 1;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");         // the tile under way too: its buffer may be filled anew
+        __syncthreads();
+        if (again) {
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) o[d][x] = 0.f;
+            m = thr = -INFINITY;
+            nm = l = 0.f;
+            kt = t0;
+            buf = 0;
+            have = 15u;
+            first = t0 * 64 >> a.shift;
+            entries = row[min(first + lane, a.width - 1)];
+            next = move(t0, 0);
+        }
     }
     for (bool here = have != 15u; kt < t1; ++kt, buf ^= 1, here = false) {
         if (!here) have = arrive();

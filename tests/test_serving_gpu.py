@@ -635,3 +635,54 @@ def test_serving_step_captured_and_replayed(dev):
         assert torch.equal(out, want), i
         for k in eager:
             assert torch.equal(eager[k], graphed[k]), (i, k)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,news,kw", [
+    ([1, 17, 40, 130, 333, 700], [1] * 6, dict(max_q=1)),                      # one token, short
+    ([1500] * 4, [1] * 4, dict(max_q=1, causal=False)),                         # frames
+    ([5001, 3000], [1, 1], dict(max_q=1)),                                      # split keys
+    ([300, 90, 500], [5, 9, 30], dict()),                                       # a few tokens
+    ([700, 520, 40], [130, 300, 2], dict()),                                    # chunks, and a request with few rows beside them
+    ([4100], [70], dict())])                                                    # a chunk with split keys
+def test_attn_bf16_is_the_exact_result_rounded_once(dev, D, lens, news, kw):
+    """Against the 64-bit result rounded to bf16.  What the kernel holds before its own rounding is off by r: the probabilities by at
+    most 2^-16 of themselves (two bf16 pieces, half a step of half a step), fp32 sums by less, and the errors are independent, so that r is
+    about 2^-16 |o|.  An element then crosses a border between two bf16 values with probability r / step and is a step off: in the mean
+    of squares r * step <= 2^-16 * 2^-7 |o|^2, a norm of 2^-11.5 = 0.09 HALF; twice that is allowed.  Probabilities of one bf16 piece would give
+    0.5 HALF."""
+    g = torch.Generator().manual_seed(D + len(lens))
+    kw = dict(kw)
+    causal = kw.pop("causal", True)
+    Hq, Hk = 4, 2
+    c = Cache(lens, Hk, D, 64, BF, g)
+    start = [0]
+    for n in news:
+        start.append(start[-1] + n)
+    q = torch.randn(start[-1], Hq, D, generator=g).to(BF)
+    kp, vp = c.views(dev)
+    got = ops.paged_attn(q.to(dev), kp, vp, c.table.to(dev), i32(lens, dev), i32(start, dev), scale=D ** -0.5, causal=causal, **kw).cpu().double()
+    want = torch.cat([attn_ref(q[start[b]:start[b + 1]], c.k[b], c.v[b], D ** -0.5, causal, BF)[0] for b in range(len(lens))])
+    assert (got - want.to(BF).double()).norm() <= 0.2 * HALF[BF] * want.norm()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 20, 200])
+def test_attn_infinite_values_with_equal_weights(dev, dtype, D, n):
+    """Queries of zeros weigh all keys alike, with a probability before normalisation of exactly 1: both infinities come through, together
+    they are NaN, and the other columns are the mean."""
+    g = torch.Generator().manual_seed(22)
+    lens = [700, 400]
+    c = Cache(lens, 1, D, 32, dtype, g)
+    kp, vp = c.views(dev)
+    q = torch.zeros(2 * n, 2, D, dtype=dtype)
+    inf = float("inf")
+    for key, d, v in ((3, 0, inf), (100, 1, -inf), (7, 2, inf), (199, 2, -inf), (64, D - 1, inf)):
+        vp[c.table[0, key // 32].item(), 0, key % 32, d] = v
+    got = ops.paged_attn(q.to(dev), kp, vp, c.table.to(dev), i32(lens, dev), i32([0, n, 2 * n], dev), scale=1.0).cpu().double()
+    rows = got[:n]
+    assert (rows[:, :, 0] == inf).all() and (rows[:, :, 1] == -inf).all() and rows[:, :, 2].isnan().all() and (rows[:, :, D - 1] == inf).all()
+    for b, keep in ((0, list(range(3, D - 1))), (1, list(range(D)))):
+        o, bound = attn_ref(q[b * n:(b + 1) * n], c.k[b], c.v[b], 1.0, True, dtype)
+        assert ((got[b * n:(b + 1) * n] - o).abs() <= bound)[:, :, keep].all()
