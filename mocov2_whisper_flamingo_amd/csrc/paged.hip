@@ -838,15 +838,19 @@ __global__ __launch_bounds__(256) void paged_attn_join_kernel(AttnArgs a) {
     float o[D / 64];
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) o[c] = 0.f;
-    for (int s0 = 0; s0 < a.splits; s0 += 8) {                 // eight loads in flight; lanes behind the last split weigh 0
+    auto add = [&](int s0, int n) {                             // n splits from s0 on
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
+        for (int u = 0; u < n; ++u) {
             const float f = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s0 + u));
-            const float* ps = p + (long)min(s0 + u, a.splits - 1) * D;
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) o[c] = fmaf(f, ps[c], o[c]);
+            for (int c = 0; c < D / 64; ++c) o[c] = fmaf(f, p[(long)(s0 + u) * D + c], o[c]);
         }
-    }
+    };
+    int s0 = 0;
+    for (; s0 + 8 <= a.splits; s0 += 8) add(s0, 8);             // eight loads in flight
+    if (a.splits & 4) { add(s0, 4); s0 += 4; }
+    if (a.splits & 2) { add(s0, 2); s0 += 2; }
+    if (a.splits & 1) add(s0, 1);
     T* out = (T*)a.o + (long)t * a.ldo + (long)h * a.ho + lane * (D / 64);
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) out[c] = from_f32<T>(o[c]);

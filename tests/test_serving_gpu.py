@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from mocov2_whisper_flamingo_amd import ops
+from mocov2_whisper_flamingo_amd import _lib, ops
 from tests.serving_ref import Cache, HALF, U32, attn_ref, plan_ref, up
 
 pytestmark = pytest.mark.gpu
@@ -686,3 +686,24 @@ def test_attn_infinite_values_with_equal_weights(dev, dtype, D, n):
     for b, keep in ((0, list(range(3, D - 1))), (1, list(range(D)))):
         o, bound = attn_ref(q[b * n:(b + 1) * n], c.k[b], c.v[b], 1.0, True, dtype)
         assert ((got[b * n:(b + 1) * n] - o).abs() <= bound)[:, :, keep].all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hit", [4599, 1000])
+def test_attn_infinite_values_in_a_split_context(dev, dtype, D, hit):
+    """A visible infinite value gives an infinity in its column, whether the keys are split or not, and whichever split it stands in."""
+    g = torch.Generator().manual_seed(21)
+    L = 4600
+    c = Cache([L], 1, D, 64, dtype, g)
+    kp, vp = c.views(dev)
+    q = torch.randn(1, 2, D, generator=g).to(dtype)
+    splits = _lib.load().avsr_paged_attn_workspace_bytes(ops._dt(q), 1, 1, 2, 1, D, 1, L) // (4 * 2 * (D + 2))
+    assert splits > 1 and splits % 8                           # the join runs in groups of eight
+    vp[c.table[0, hit // 64].item(), 0, hit % 64, 5] = float("inf")
+    o, bound = attn_ref(q, c.k[0], c.v[0], D ** -0.5, True, dtype)
+    for mk in (L, 512):
+        got = ops.paged_attn(q.to(dev), kp, vp, c.table.to(dev), i32([L], dev), i32([0, 1], dev), max_q=1, max_k=mk, scale=D ** -0.5).cpu().double()
+        assert (got[:, :, 5] == float("inf")).all(), mk
+        keep = [d for d in range(D) if d != 5]
+        assert ((got - o).abs() <= bound)[:, :, keep].all()
