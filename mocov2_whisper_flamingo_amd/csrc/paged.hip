@@ -1292,6 +1292,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
 struct AttnPlan { bool ahead; int waves, splits, tiles_few, few_rows, chunk_rows; bool few, chunk; int64_t chunk_tiles, grid_few, grid_chunk, floats; };
 static AttnPlan attn_plan(int dtype, int64_t D, int64_t N, int64_t B, int64_t Hk, int64_t G, int64_t max_q, int64_t max_k) {
     AttnPlan p;
+    if (max_q > N) max_q = N;                                  // here, so that the size query and the call make one plan of one bound
     const int64_t rows = max_q * G;
     p.chunk = rows > FEW_ROWS;
     p.few = !(p.chunk && B == 1 && N * G > FEW_ROWS);          // one large request: nothing for the first kernel
@@ -1366,8 +1367,8 @@ extern "C" int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, i
         ((uintptr_t)q | (uintptr_t)k_pages | (uintptr_t)v_pages | (uintptr_t)o) % 16) return AVSR_EUNSUPPORTED;
     if (N > (1 << 28) || N * Hq > (1LL << 30) || B > (1 << 24) || B * Hk > (1LL << 24)) return AVSR_EUNSUPPORTED;
     if (N == 0) return AVSR_OK;
-    const int64_t mq = max_q < N ? max_q : N, mk = max_k < width * page ? max_k : width * page;
-    const AttnPlan p = attn_plan(dtype, head_dim, N, B, Hk, Hq / Hk, mq, mk);
+    const int64_t mk = max_k < width * page ? max_k : width * page;       // fewer keys are never split more
+    const AttnPlan p = attn_plan(dtype, head_dim, N, B, Hk, Hq / Hk, max_q, mk);
     if (p.floats && (!workspace || workspace_bytes < p.floats * 4 || (uintptr_t)workspace % 16)) return AVSR_EINVAL;
     const int64_t n_few = p.chunk ? p.grid_few * p.tiles_few : 0;
     // a launch has fewer than 2^32 threads

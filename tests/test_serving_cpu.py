@@ -192,3 +192,22 @@ def test_plan_restatement_keeps_every_page_once():
         held = [table[b][j] for b in range(B) for j in range(up(lens[b], page))]
         free = [ring[(pool[0] + i) % n] for i in range(pool[1])]
         assert sorted(held + free) == list(range(n))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_attn_workspace_of_a_general_bound(dtype, D):
+    """A bound for any step (max_q above the rows of this one) asks for what the tight one does, and fewer keys never for more: what the
+    query says is enough for the call, whatever it knows besides."""
+    size = _lib.load().avsr_paged_attn_workspace_bytes
+    for N, B, Hq, Hk, k in ((4, 4, 32, 8, 8000), (1, 1, 20, 20, 4000), (8, 3, 12, 12, 1500), (70, 2, 16, 4, 30000), (2, 2, 7, 1, 700)):
+        tight = size(dtype, N, B, Hq, Hk, D, N, k)
+        assert tight > 0
+        for q in (N + 1, 65, 448, 1 << 40):
+            if q > N:
+                assert size(dtype, N, B, Hq, Hk, D, q, k) == tight
+        most = 0
+        for fewer in range(1, k + 1, 37):
+            here = size(dtype, N, B, Hq, Hk, D, 1, fewer)
+            assert here >= most
+            most = here

@@ -707,3 +707,24 @@ def test_attn_infinite_values_in_a_split_context(dev, dtype, D, hit):
         assert (got[:, :, 5] == float("inf")).all(), mk
         keep = [d for d in range(D) if d != 5]
         assert ((got - o).abs() <= bound)[:, :, keep].all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attn_c_entry_takes_the_workspace_it_asks_for(dev, dtype, D):
+    """Bounds for any step of a server (max_q far above the rows of this one): the entry works in what the query said, and gives what it
+    gives with tight bounds."""
+    g = torch.Generator().manual_seed(D)
+    lens, Hq, Hk, lib = [5000, 8000, 17, 900], 32, 8, _lib.load()
+    c = Cache(lens, Hk, D, 64, dtype, g)
+    kp, vp = c.views(dev)
+    q, table = torch.randn(4, Hq, D, generator=g).to(dtype).to(dev), c.table.to(dev)
+    held, start = i32(lens, dev), i32([0, 1, 2, 3, 4], dev)
+    want = ops.paged_attn(q, kp, vp, table, held, start, max_q=4, max_k=8000, scale=D ** -0.5)
+    dt, out = ops._dt(q), torch.zeros_like(q)
+    size = lib.avsr_paged_attn_workspace_bytes(dt, 4, 4, Hq, Hk, D, 448, 8000)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+    rc = lib.avsr_paged_attn(torch.cuda.current_stream().cuda_stream, dt, q.data_ptr(), Hq * D, D, kp.data_ptr(), kp.stride(0), kp.stride(1), vp.data_ptr(),
+                             vp.stride(0), vp.stride(1), table.data_ptr(), table.stride(0), table.shape[1], held.data_ptr(), start.data_ptr(),
+                             out.data_ptr(), Hq * D, D, 4, 4, Hq, Hk, D, 64, kp.shape[0], 448, 8000, D ** -0.5, 1, ws.data_ptr(), size)
+    assert rc == 0 and torch.equal(out, want)
