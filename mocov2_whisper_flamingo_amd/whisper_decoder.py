@@ -274,6 +274,14 @@ class WhisperDecoder(nn.Module):
                                                 pages=requests * -(-most // page_size) if count is None else count)
         return PagedDecoderCache(make(n, pages), None if frames is None else make(int(frames), frame_pages), dtype, device)
 
+    def _own_cache(self, cache):
+        """Refuses a cache that was made for another decoder, before anything of it moves on."""
+        H, kv = self.cfg.decoder_attention_heads, cache.tokens.kv
+        if len(kv) != len(self.layers) or tuple(kv[0].shape[2::2]) != (H, self.cfg.d_model // H):
+            raise ValueError("the cache is another decoder's: its layers, heads or head size differ")
+        if self.embed_tokens.weight.device != cache.bad.device:
+            raise ValueError("the cache is not on the decoder's device")
+
     @torch.no_grad()
     def paged_admit(self, cache, requests, encoder_hidden_states):
         """Encoder output [n, Te, D] of the n given requests (ascending, none of which holds frames) into the cache's frames.  Raises
@@ -281,6 +289,7 @@ class WhisperDecoder(nn.Module):
         if cache.frames is None:
             raise ValueError("the cache was made without frames")
         requests = [int(r) for r in requests]
+        self._own_cache(cache)
         n, Te, D = encoder_hidden_states.shape
         if D != self.cfg.d_model or encoder_hidden_states.device != cache.bad.device or Te == 0:
             raise ValueError(f"paged_admit expects encoder output [n, frames, {self.cfg.d_model}] on the cache's device")
@@ -310,8 +319,11 @@ class WhisperDecoder(nn.Module):
         at most so many new tokens of one request; default N): ``plan.status`` and ``cache.bad`` say whether it went well; rows behind
         the last token hold nothing."""
         cfg, dtype, tok = self.cfg, cache.dtype, cache.tokens
-        if input_ids.dim() != 1 or input_ids.dtype != torch.int64:
-            raise ValueError("input_ids must be int64 [tokens]")
+        H, D, dev = cfg.decoder_attention_heads, cfg.d_model, cache.bad.device
+        # all that can be wrong is looked at here: the plan below moves the cache on
+        if input_ids.dim() != 1 or input_ids.dtype != torch.int64 or input_ids.device != dev:
+            raise ValueError("input_ids must be int64 [tokens] on the cache's device")
+        self._own_cache(cache)
         N = input_ids.shape[0]
         checked = not torch.is_tensor(new)
         if checked:
@@ -321,14 +333,17 @@ class WhisperDecoder(nn.Module):
             if N and bool(((input_ids < 0) | (input_ids >= cfg.vocab_size)).any()):
                 raise IndexError("token id out of range for the embedding table")
             max_new = max(new)
-            new = torch.tensor(new, dtype=torch.int32, device=cache.bad.device)
+            new = torch.tensor(new, dtype=torch.int32, device=dev)
+        elif new.dtype != torch.int32 or new.shape != tok.lens.shape or new.device != dev or not new.is_contiguous():
+            raise ValueError(f"new must be a contiguous int32 tensor of {tok.requests} values on the cache's device")
+        elif max_new is not None and max_new < 1:
+            raise ValueError("max_new must be positive")
         pk = self._pack(dtype)
         plan = tok.plan(new, max(N, 1))
         if checked:
             tok.check(plan)
-        H, D = cfg.decoder_attention_heads, cfg.d_model
         if N == 0:
-            return torch.empty((0, D), dtype=dtype, device=input_ids.device), plan
+            return torch.empty((0, D), dtype=dtype, device=dev), plan
         heads = lambda t: t.unflatten(1, (H, -1))
         xs = ops.embed_tokens_at(input_ids, pk["tok"], pk["pos"], plan.positions, bad=cache.bad)
         for i, lw in enumerate(pk["layers"]):

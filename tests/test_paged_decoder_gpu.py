@@ -248,3 +248,36 @@ def test_paged_step_captured_and_replayed(dev, group):
         assert torch.equal(nxt[:rows], dec.project_tokens(want[None]).view(R, -1)[:rows])
         assert graphed.tokens.lens.tolist() == eager.tokens.lens.tolist()
     assert graphed.bad.item() == 0
+
+
+def test_calls_that_are_refused_leave_the_cache_as_it_was(dev):
+    """Everything that can be wrong with a step is looked at before the cache moves on."""
+    dec, sd, cfg = model(dev)
+    cache = dec.new_paged_cache(2, page_size=16, max_tokens=48)
+    ids = torch.arange(3, 43, device=dev)
+    dec.paged_step(cache, ids[:12], [7, 5])
+    state = lambda: [t.tolist() for t in (cache.tokens.lens, cache.tokens.table, cache.tokens.ring, cache.tokens.pool)]
+    before, one = state(), torch.ones(2, dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError):
+        dec.paged_step(cache, ids[:2].cpu(), [1, 1])
+    with pytest.raises(ValueError):
+        dec.paged_step(cache, ids[:2].cpu(), one, max_new=1)
+    for bad in (0, -1):
+        with pytest.raises(ValueError):
+            dec.paged_step(cache, ids[:2], one, max_new=bad)
+    for new in (one.cpu(), one.long(), one[:1], torch.ones(3, dtype=torch.int32, device=dev)):
+        with pytest.raises(ValueError):
+            dec.paged_step(cache, ids[:2], new, max_new=1)
+    for other in (model(dev, d=192, heads=3)[0], WhisperModel(WhisperConfig(d_model=128, decoder_layers=3, decoder_attention_heads=2, vocab_size=VOCAB,
+                                                                            max_target_positions=448)).to(dev).decoder):
+        with pytest.raises(ValueError):
+            other.paged_step(cache, ids[:2], [1, 1])
+        framed = other.new_paged_cache(2, page_size=16, frames=16)
+        with pytest.raises(ValueError):
+            dec.paged_admit(framed, [0], torch.zeros(1, 16, cfg.d_model, device=dev))
+        assert framed.frames.lens.tolist() == [0, 0]
+    assert state() == before
+    seq = torch.cat([ids[:7], ids[20:21]]).cpu()
+    h, _ = dec.paged_step(cache, ids[20:22], [1, 1])
+    ref = oracle.whisper_decoder(sd, "decoder.", seq[None], None, 2)[0]
+    assert max_err(h[:1], ref[-1:]) < TOL[torch.bfloat16]
