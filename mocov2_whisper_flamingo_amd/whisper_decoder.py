@@ -314,10 +314,12 @@ class WhisperDecoder(nn.Module):
         go with :meth:`paged_end`); ``input_ids`` int64 [N]: these tokens, request after request.  Returns their hidden states [N, D],
         the values :meth:`forward` gives for these positions of each request's sequence, and the step's plan.
 
-        ``new`` as a list is checked: the call waits for the GPU, and raises, with nothing changed, on ids outside the vocabulary and on
-        a step that does not fit.  As an int32 GPU tensor it is taken as it is, and the call can be recorded in a HIP graph (``max_new``:
-        at most so many new tokens of one request; default N): ``plan.status`` and ``cache.bad`` say whether it went well; rows behind
-        the last token hold nothing."""
+        ``new`` as a list is checked: the call waits for the GPU, and raises, with nothing changed, on ids outside the vocabulary, on
+        a step that does not fit, and (with a cache for frames) on tokens of a request that was not admitted.  As an int32 GPU tensor it
+        is taken as it is, and the call can be recorded in a HIP graph (``max_new``: at most so many new tokens of one request; default
+        N): ``plan.status`` and ``cache.bad`` say whether it went well; rows behind the last token hold nothing, but their ids are looked
+        up too, so any of the vocabulary stands there; whether a request holds frames is the caller's to know
+        (``cache.frames.lens``): without any it attends to nothing."""
         cfg, dtype, tok = self.cfg, cache.dtype, cache.tokens
         H, D, dev = cfg.decoder_attention_heads, cfg.d_model, cache.bad.device
         # all that can be wrong is looked at here: the plan below moves the cache on
@@ -332,6 +334,8 @@ class WhisperDecoder(nn.Module):
                 raise ValueError(f"new must give each of the {tok.requests} requests its share of the {N} tokens")
             if N and bool(((input_ids < 0) | (input_ids >= cfg.vocab_size)).any()):
                 raise IndexError("token id out of range for the embedding table")
+            if N and cache.frames is not None and any(n > 0 and not held for n, held in zip(new, cache.frames.lens.tolist())):
+                raise ValueError("a request that adds tokens holds no frames: paged_admit first")
             max_new = max(new)
             new = torch.tensor(new, dtype=torch.int32, device=dev)
         elif new.dtype != torch.int32 or new.shape != tok.lens.shape or new.device != dev or not new.is_contiguous():

@@ -281,3 +281,20 @@ def test_calls_that_are_refused_leave_the_cache_as_it_was(dev):
     h, _ = dec.paged_step(cache, ids[20:22], [1, 1])
     ref = oracle.whisper_decoder(sd, "decoder.", seq[None], None, 2)[0]
     assert max_err(h[:1], ref[-1:]) < TOL[torch.bfloat16]
+
+
+def test_requests_without_frames_are_refused(dev):
+    """With a cache for frames, a request that was not admitted (or was not again after its end) has nothing to attend to."""
+    dec, sd, cfg = model(dev)
+    cache = dec.new_paged_cache(3, frames=20, page_size=16, max_tokens=48)
+    enc, ids = torch.randn(1, 20, cfg.d_model, device=dev), torch.arange(3, 10, device=dev)
+    dec.paged_admit(cache, [1], enc)
+    with pytest.raises(ValueError, match="admit"):
+        dec.paged_step(cache, ids[:4], [2, 2, 0])
+    assert cache.tokens.lens.tolist() == [0, 0, 0]
+    dec.paged_step(cache, ids[:2], [0, 2, 0])
+    dec.paged_end(cache, [1])
+    with pytest.raises(ValueError, match="admit"):
+        dec.paged_step(cache, ids[:2], [0, 2, 0])
+    assert cache.tokens.lens.tolist() == [0, 0, 0]
+    dec.paged_step(cache, ids[:0], [-1, 0, -1])                 # ends and waits need no frames
