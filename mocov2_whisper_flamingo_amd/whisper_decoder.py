@@ -261,13 +261,19 @@ class WhisperDecoder(nn.Module):
     # ---- requests of different lengths ---------------------------------------
     def new_paged_cache(self, requests, *, pages=None, page_size=64, max_tokens=None, frames=None, frame_pages=None, dtype=torch.bfloat16,
                         device=None):
-        """An empty cache for ``requests`` requests of up to ``max_tokens`` tokens (default and most: max_target_positions) over ``pages``
-        pages (default: enough for all of them).  ``frames``: most encoder frames of a request, over ``frame_pages`` pages; None: no
-        cross-attention."""
+        """An empty cache for ``requests`` requests of up to ``max_tokens`` tokens over ``pages`` pages (default: enough for all of them).
+        ``max_tokens`` is a multiple of the page size, so that the plan keeps to it: max_target_positions at most, which is also the
+        default; where that is no multiple (448 with pages of 128 or 256), it has to be given.  ``frames``: most encoder frames of a
+        request, over ``frame_pages`` pages; None: no cross-attention."""
+        most = self.cfg.max_target_positions
+        n = most if max_tokens is None else int(max_tokens)
+        if n > most or n < 1 or n % page_size:
+            raise ValueError(f"max_tokens must be given as a multiple of the page size {page_size}, up to max_target_positions={most}")
+        return self._paged_cache(requests, n, pages, page_size, frames, frame_pages, dtype, device)
+
+    def _paged_cache(self, requests, n, pages, page_size, frames, frame_pages, dtype, device):
+        """Without the check: a caller that keeps to max_target_positions itself may have its last page reach beyond."""
         cfg = self.cfg
-        n = cfg.max_target_positions if max_tokens is None else int(max_tokens)
-        if n > cfg.max_target_positions or n < 1 or n % page_size:
-            raise ValueError(f"max_tokens must be a multiple of the page size, up to max_target_positions={cfg.max_target_positions}")
         device = device or self.embed_tokens.weight.device
         H, D = cfg.decoder_attention_heads, cfg.d_model // cfg.decoder_attention_heads
         make = lambda most, count: PagedKVCache(len(self.layers), requests, H, D, max_tokens=most, page_size=page_size, dtype=dtype, device=device,
@@ -382,15 +388,15 @@ class WhisperDecoder(nn.Module):
     @torch.no_grad()
     def greedy_ragged(self, prompts, encoder_hidden_states, max_new_tokens, eos_token_id=None, dtype=torch.bfloat16, page_size=64):
         """Greedy decoding of prompts of different lengths (lists of token ids, none empty) in one ragged batch: each prompt's list with
-        what was generated, up to ``max_new_tokens`` or its own ``eos_token_id``.  A request that is done gives its tokens' pages back in the next step."""
-        R = len(prompts)
+        what was generated, up to ``max_new_tokens``, its own ``eos_token_id`` or max_target_positions cached tokens.  A request that is done
+        gives its tokens' pages back in the next step."""
+        R, most = len(prompts), self.cfg.max_target_positions
         out = [[int(t) for t in p] for p in prompts]
-        if R == 0 or any(not p for p in out):
-            raise ValueError("greedy_ragged expects prompts of at least one token")
+        if R == 0 or any(not 0 < len(p) <= most for p in out):
+            raise ValueError(f"greedy_ragged expects prompts of 1 to max_target_positions={most} tokens")
         dev = encoder_hidden_states.device
-        cache = self.new_paged_cache(R, page_size=page_size, frames=encoder_hidden_states.shape[1], dtype=dtype, device=dev)
+        cache = self._paged_cache(R, most, None, page_size, encoder_hidden_states.shape[1], None, dtype, dev)
         self.paged_admit(cache, range(R), encoder_hidden_states)
-        most = self.cfg.max_target_positions
         ids, new, left = [t for p in out for t in p], [len(p) for p in out], [max_new_tokens] * R
         while any(n > 0 for n in new):
             h, _ = self.paged_step(cache, torch.tensor(ids, dtype=torch.int64, device=dev), new)

@@ -298,3 +298,21 @@ def test_requests_without_frames_are_refused(dev):
         dec.paged_step(cache, ids[:2], [0, 2, 0])
     assert cache.tokens.lens.tolist() == [0, 0, 0]
     dec.paged_step(cache, ids[:0], [-1, 0, -1])                 # ends and waits need no frames
+
+
+@pytest.mark.parametrize("page_size", [16, 64, 128, 256])
+@pytest.mark.parametrize("positions", [448, 100])
+def test_greedy_ragged_takes_every_page_size(dev, page_size, positions):
+    """Also where the positions are no multiple of it; and the limits of the length are those of greedy."""
+    cfg = WhisperConfig(d_model=128, decoder_layers=2, decoder_attention_heads=2, vocab_size=VOCAB, max_target_positions=positions)
+    m = WhisperModel(cfg)
+    seed_module(m, 61)
+    dec = m.to(dev).decoder
+    g = torch.Generator().manual_seed(8)
+    prompts = [torch.randint(3, VOCAB, (n,), generator=g).tolist() for n in (4, positions - 3, positions, 30)]
+    enc = torch.randn(4, 30, cfg.d_model, generator=g).to(dev)
+    want = [dec.greedy(torch.tensor([p], device=dev), enc[i:i + 1], 9, dtype=torch.float32)[0].tolist() for i, p in enumerate(prompts)]
+    got = dec.greedy_ragged(prompts, enc, 9, dtype=torch.float32, page_size=page_size)
+    assert got == want and [len(w) for w in want] == [13, positions + 1, positions + 1, 39]
+    with pytest.raises(ValueError):
+        dec.greedy_ragged([prompts[0], [5] * (positions + 1)], enc[:2], 2, dtype=torch.float32, page_size=page_size)
