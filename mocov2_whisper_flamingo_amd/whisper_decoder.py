@@ -394,6 +394,8 @@ class WhisperDecoder(nn.Module):
         out = [[int(t) for t in p] for p in prompts]
         if R == 0 or any(not 0 < len(p) <= most for p in out):
             raise ValueError(f"greedy_ragged expects prompts of 1 to max_target_positions={most} tokens")
+        if max_new_tokens < 1:
+            return out
         dev = encoder_hidden_states.device
         cache = self._paged_cache(R, most, None, page_size, encoder_hidden_states.shape[1], None, dtype, dev)
         self.paged_admit(cache, range(R), encoder_hidden_states)
@@ -405,9 +407,6 @@ class WhisperDecoder(nn.Module):
             nxt = ops.argmax_rows(self.project_tokens(h[last][:, None]).view(len(live), -1)).tolist()
             ids, new = [], [0] * R
             for r, t in zip(live, nxt):
-                if left[r] == 0:
-                    new[r] = -1
-                    continue
                 out[r].append(t)
                 left[r] -= 1
                 done = left[r] == 0 or t == eos_token_id or len(out[r]) > most

@@ -316,3 +316,10 @@ def test_greedy_ragged_takes_every_page_size(dev, page_size, positions):
     assert got == want and [len(w) for w in want] == [13, positions + 1, positions + 1, 39]
     with pytest.raises(ValueError):
         dec.greedy_ragged([prompts[0], [5] * (positions + 1)], enc[:2], 2, dtype=torch.float32, page_size=page_size)
+
+
+@pytest.mark.parametrize("most", [0, -1, -5])
+def test_greedy_ragged_adds_nothing_for_no_tokens(dev, most):
+    dec, sd, cfg = model(dev)
+    enc = torch.zeros(2, 16, cfg.d_model, device=dev)
+    assert dec.greedy_ragged([[5, 6], [7]], enc, most, dtype=torch.float32) == [[5, 6], [7]]
