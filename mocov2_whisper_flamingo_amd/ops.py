@@ -1167,8 +1167,9 @@ def w4_pack(q, scales, group):
         raise ValueError("w4_pack expects whole numbers [N, K] and scales [N, ceil(K / group)]")
     if int(q.min()) < -8 or int(q.max()) > 7:
         raise ValueError("4-bit weights lie in -8 .. 7")
+    scales = scales.to(torch.bfloat16)
     if not bool(torch.isfinite(scales).all()):
-        raise ValueError("scales must be finite")
+        raise ValueError("scales must be finite in bf16")
     N, K = q.shape
     T, C = -(-N // 16), -(-K // 128)
     full = torch.zeros((T * 16, C * 128), dtype=torch.int32, device=q.device)

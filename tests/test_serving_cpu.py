@@ -211,3 +211,14 @@ def test_attn_workspace_of_a_general_bound(dtype, D):
             here = size(dtype, N, B, Hq, Hk, D, 1, fewer)
             assert here >= most
             most = here
+
+
+@pytest.mark.parametrize("scale", [torch.tensor(3.4e38), -torch.tensor(3.4e38), torch.tensor(1e300, dtype=torch.float64)])
+def test_w4_scales_have_to_stay_finite_in_bf16(scale):
+    """Finite in the caller's type, but beyond the largest bf16 value (3.39e38): they would be infinite in the packed weights."""
+    s = torch.ones(3, 2, dtype=scale.dtype)
+    s[1, 1] = scale
+    with pytest.raises(ValueError, match="finite"):
+        ops.w4_pack(z(3, 40), s, 32)
+    s[1, 1] = scale.sign() * 3.38e38
+    assert torch.isfinite(ops.w4_pack(z(3, 40), s, 32).scales).all()
