@@ -728,3 +728,19 @@ def test_attn_c_entry_takes_the_workspace_it_asks_for(dev, dtype, D):
                              vp.stride(0), vp.stride(1), table.data_ptr(), table.stride(0), table.shape[1], held.data_ptr(), start.data_ptr(),
                              out.data_ptr(), Hq * D, D, 4, 4, Hq, Hk, D, 64, kp.shape[0], 448, 8000, D ** -0.5, 1, ws.data_ptr(), size)
     assert rc == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,news,page", [([1500, 1100], [130, 70], 16), ([2500, 64, 2100], [100, 40, 1], 16), ([4300], [150], 32)])
+def test_attn_chunks_over_long_tables(dev, dtype, D, lens, news, page):
+    """Chunks of requests with more than 64 entries in the block table, keys split and not.  The bound of every element grows with the
+    length; as a whole, the result is the exact one to HALF / sqrt(3) (a uniform rounding of a value at the lower end of its octave) and
+    fp32 noise of 2^-16, while one key of 4300 is a part of 1 / sqrt(4300) = 0.015 in it."""
+    got = attend_and_check(dev, lens, news, 4, 2, D, page, dtype, True, seed=31)
+    g = torch.Generator().manual_seed(31)
+    c = Cache(lens, 2, D, page, dtype, g)
+    start = [sum(news[:b]) for b in range(len(news) + 1)]
+    q = torch.randn(start[-1] + 3, 4, 2 * D, generator=g).to(dtype)[:, :, D:]
+    want = torch.cat([attn_ref(q[start[b]:start[b + 1]], c.k[b], c.v[b], D ** -0.5, True, dtype)[0] for b in range(len(lens))])
+    assert (got.double() - want).norm() <= (0.6 * HALF[dtype] + 2.0 ** -16) * want.norm()
