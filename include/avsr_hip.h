@@ -578,7 +578,7 @@ int avsr_paged_write(avsr_stream_t stream, int in_dtype, int page_dtype, const v
  * yields zeros; rows behind q_start[B] are left as they were; a key that a row does not see has no influence on it,
  * whatever it holds; a table entry that names no page hides its keys.  Softmax statistics and sums in fp32; with
  * bf16 the probabilities enter the second product as two bf16 values each (2^-16 of themselves).  max_q, max_k: at most so many new tokens and keys in any request;
- * they choose the grid, larger requests still come out right.  o may be q.  Results do not depend on the workspace's contents. */
+ * they choose the grid, larger requests still come out right.  o may be q (the same strides) and overlaps nothing else.  Results do not depend on the workspace's contents. */
 int64_t avsr_paged_attn_workspace_bytes(int dtype, int64_t N, int64_t B, int64_t Hq, int64_t Hk, int64_t head_dim,
                                         int64_t max_q, int64_t max_k);
 int avsr_paged_attn(avsr_stream_t stream, int dtype, const void* q, int64_t ldq, int64_t q_head, const void* k_pages,
@@ -597,7 +597,7 @@ int avsr_embed_tokens_at(avsr_stream_t stream, int table_dtype, const int64_t* i
  * word[n/16][k/128][k/8 % 4][n % 16][k/32 % 4], the nibble of k % 8 = e at bit 4*(e/2) + 16*(e%2); scales: bf16
  * [n/16][k/group][n % 16]; both padded to whole tiles of 16 rows and 128 columns with nibble 8 and scale 0.
  * group: 32, 64 or 128; M up to 2^19, N to 2^28, K to 2^24.  x fp32 or bf16, y and residual fp32 or bf16 (residual of y's
- * type, may be y itself); act NONE, GELU or RELU.  fp32 sums, which pass through some thousand times the largest x: it is at
+ * type, may be y itself; else y overlaps nothing); act NONE, GELU or RELU.  fp32 sums, which pass through some thousand times the largest x: it is at
  * most 1e34 in magnitude.  A row of x with a value that is not finite yields NaN. */
 int avsr_w4_matmul(avsr_stream_t stream, int x_dtype, int out_dtype, const void* x, int64_t ldx, const void* packed,
                    const void* scales, int64_t group, const float* bias, int act, const void* residual, int64_t ldr,

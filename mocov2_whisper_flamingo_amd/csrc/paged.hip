@@ -736,9 +736,10 @@ template <int D> __device__ __forceinline__ void store_vals(float* p, const floa
 
 // ---- few rows: the WAVES waves of a workgroup take the tiles of the keys in turn and are merged through LDS; a split
 // grid leaves {m, l} and O of every row and split to paged_attn_join_kernel.  One row would do with vector instructions, but
-// 16 cost the matrix pipe nothing that the memory would not take longer for: 64 requests x 20 heads x 1500 keys (492 MB) in
-// 85 us, 5.8 TB/s, the rate of a long read; 4 requests of 7000 to 32700 keys, 8 heads of 128 (271 MB), 56 us and 5 for the
-// join; 8 requests x 6 heads x 440 keys 7 us, a launch and three dependent trips to memory.
+// 16 cost the matrix pipe nothing that the memory would not take longer for, probabilities in two pieces included (one piece: the same
+// times, 0.4 us less for the smallest): 64 requests x 20 heads x 1500 keys (492 MB) in 86 us, 5.7 TB/s, the rate of a long read;
+// 4 requests of 7000 to 32700 keys, 8 heads of 128 (271 MB), 56 us and 5 for the join; 8 requests x 6 heads x 440 keys 7.5 us, a
+// launch and three dependent trips to memory.
 template <int D, int WAVES> struct FewLds { float m[WAVES][16], l[WAVES][16], o[WAVES][16][D + 4]; };
 template <typename T, int D, int WAVES, bool AHEAD>
 __device__ __forceinline__ void attn_few(const AttnArgs& a, FewLds<D, WAVES>& lds, int bx, int by, int ny) {
@@ -953,9 +954,9 @@ __global__ __launch_bounds__(256) void paged_attn_rows_kernel(AttnArgs a) {
 // 4096 keys, 16 heads over 4: 241 us (535 TF) with 64 columns, 200 us (645 TF) with 8 heads of 128.  With probabilities of one bf16
 // value, two products of three, 169 and 148 us.
 // Requests with few rows, bound by memory, are in the same grid: beside the matrix products of the others (64 requests of 1 to 512
-// tokens on 1000 to 4000 keys, 16 heads over 4: 65 us, as two launches 100; 32 of 1 to 1000 on up to 6000, 32 heads of 128 over
-// 8: 173, 226).  They start behind as many of the large ones as fill half the chip's places, which then lie evenly on the CUs: in
-// front of all of them 64 requests of 1 to 224 tokens take 37 us, behind them 29 but the batch of 32 227, here 29 and 173.
+// tokens on 1000 to 4000 keys, 16 heads over 4: 82 us, as two launches 119; 32 of 1 to 1000 on up to 6000, 32 heads of 128 over
+// 8: 209, 266).  They start behind as many of the large ones as fill half the chip's places, which then lie evenly on the CUs: in
+// front of all of them 64 requests of 1 to 224 tokens take 40 us, behind them 32 but the batch of 32 261, here 29 and 209.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -1287,7 +1288,7 @@ __global__ __launch_bounds__(256, D == 64 ? 4 : 2) void paged_attn_chunk_kernel(
 }
 
 // Requests of up to FEW_ROWS rows (tokens times the heads that share a kv head) go to the first kernel: 16 requests of 500 to
-// 4000 keys, 64 rows each, 24.9 us there and 26.1 in the second, 128 rows 44.7 and 30.6.
+// 4000 keys, 64 rows each, 26.9 us there and 27.8 in the second, 128 rows 45.9 and 32.1.
 #define FEW_ROWS 64
 struct AttnPlan { bool ahead; int waves, splits, tiles_few, few_rows, chunk_rows; bool few, chunk; int64_t chunk_tiles, grid_few, grid_chunk, floats; };
 static AttnPlan attn_plan(int dtype, int64_t D, int64_t N, int64_t B, int64_t Hk, int64_t G, int64_t max_q, int64_t max_k) {
@@ -1302,15 +1303,15 @@ static AttnPlan attn_plan(int dtype, int64_t D, int64_t N, int64_t B, int64_t Hk
     p.chunk_tiles = p.chunk ? N * G / p.chunk_rows + B : 0;
     // Key splits where the row tiles do not fill the chip (256 CUs).  The first kernel is given up to 768 workgroups of four
     // waves (three fit on a CU; where a key takes more than 128 bytes, two fit, and twice as many even out ragged lengths:
-    // 32 requests of 1000 to 8000 keys, 8 heads of 128, 104 -> 95 us), of 128 keys at least; up to 512 keys are not split, the
+    // 32 requests of 1000 to 8000 keys, 8 heads of 128, 107 -> 95 us), of 128 keys at least; up to 512 keys are not split, the
     // join would cost more (3 us of 10).  The second kernel: up to 512 workgroups of 256 keys at least.
     const int64_t wgs = p.chunk ? Hk * p.chunk_tiles : B * Hk * p.tiles_few, bytes = D * (dtype == AVSR_F32 ? 4 : 2);
     const int64_t fill = (p.chunk ? 512 : bytes <= 128 ? 768 : 1536) / wgs, most = p.chunk ? (max_k + 255) / 256 : max_k <= 512 ? 1 : (max_k + 127) / 128;
     const int64_t s = fill < most ? fill : most;
     p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
     // Eight waves where the workgroups leave CUs free.  The next tile ahead of time where a wave has a long way to go (64
-    // requests x 20 heads of 1500 keys 91 -> 85 us) or all workgroups run at once anyway (40 requests x 8 heads of 60 to 448 keys
-    // 11.2 -> 10.2 us); with more and short ones, more waves are better (64 x 20 of 20 to 440 keys 14.1 us, 16 ahead).  Only 128
+    // requests x 20 heads of 1500 keys 92 -> 86 us) or all workgroups run at once anyway (40 requests x 8 heads of 60 to 448 keys
+    // 11.2 -> 10.4 us); with more and short ones, more waves are better (64 x 20 of 20 to 440 keys 15.1 us, 17 ahead).  Only 128
     // bytes a key leave registers for it.
     const int64_t rows_tiles = B * p.tiles_few < N * G / 16 + B ? B * p.tiles_few : N * G / 16 + B;
     p.waves = p.few && wgs * p.splits <= 256 ? 8 : 4;

@@ -1117,7 +1117,7 @@ def paged_attn(q, k_pages, v_pages, table, lens, q_start, *, max_q=None, max_k=N
     q_start[b+1]-1 are the last tokens of request b, ``lens`` [B] counts its tokens with them; ``causal=False``: each row sees all
     of them (cross-attention).  Hq is a multiple of the pages' heads.  ``max_q`` / ``max_k``: at most so many new tokens / keys in a
     request - they choose how the work is split, larger requests still come out right.  Rows behind the last request are left as
-    they are.  ``out`` may be q."""
+    they are.  ``out`` may be q, and overlaps nothing else."""
     n, Hk, page, D, kp, kh, vp, vh = _pages(k_pages, v_pages)
     shape = q.shape
     if len(shape) != 3 or shape[2] != D or shape[1] == 0 or shape[1] % Hk or q.dtype is not k_pages.dtype:
@@ -1211,8 +1211,9 @@ def _rows(t, M, N, dtype, what):
 
 def w4_matmul(x, w, *, bias=None, act=ACT_NONE, residual=None, out=None, out_dtype=None):
     """act(x @ w^T + bias) + residual for x [M, K] (fp32 or bf16) and a ``W4Weight``: [M, N] of ``out_dtype`` (x's type).
-    ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself.  x is at most 1e34 in
-    magnitude: a sum passes through some thousand times that, and a row of x with an infinity or NaN is NaN throughout."""
+    ``act``: ACT_NONE, ACT_GELU or ACT_RELU; ``residual`` of the result's type, which may be ``out`` itself; else ``out`` overlaps
+    nothing.  x is at most 1e34 in magnitude: a sum passes through some thousand times that, and a row of x with an infinity or NaN
+    is NaN throughout."""
     packed, scales, N, K, group = w
     T, C = (N + 15) // 16, (K + 127) // 128
     if (group not in W4_GROUPS or packed.dtype is not torch.int32 or packed.numel() != T * C * 256 or scales.dtype is not torch.bfloat16
